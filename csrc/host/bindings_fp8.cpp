@@ -1,0 +1,172 @@
+// Bindings of the ops that keep keys, values and normed rows in 8 bits.  As in bindings.cpp every argument is checked here (device, type,
+// contiguity, shapes, alignment), so a malformed call raises in Python instead of reaching a kernel.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/extension.h>
+
+#include <cstdint>
+
+#include "checks.h"
+
+extern "C" {
+int forge_fp8_store(const void* qkv, long long ld, const void* qw, const void* kw, float eps, const float* rope, int rope_rows,
+                    const int* positions, const int* slots, void* q_out, void* k_codes, void* k_scales, void* v_codes, void* v_scales, int T,
+                    int nq, int nkv, int block_size, long long num_slots, unsigned* status, cudaStream_t stream);
+int forge_fp8_expand(const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales, const int* block_tables,
+                     const int* lens, int num_seqs, int table_width, int num_blocks, int nkv, int block_size, void* k_out, void* v_out,
+                     int* tables, int capacity, unsigned* status, cudaStream_t stream);
+int forge_decode_fp8(const void* q, const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales,
+                     const int* block_tables, const int* lens, void* out, int B, int nq, int nkv, int block_size, int table_width,
+                     int num_blocks, float scale, unsigned* status, cudaStream_t stream);
+int forge_rms_norm_fp8(const void* x, void* residual, const void* w, void* codes, float* scales, int scale_ld, int rows, int H, float eps,
+                       cudaStream_t stream);
+}
+
+namespace {
+
+constexpr auto BF = at::kBFloat16;
+constexpr auto U8 = at::kByte;
+
+void same_device(const Tensor& a, const Tensor& b, const char* what) { TORCH_CHECK(a.device() == b.device(), what, ": tensors on one device expected"); }
+void aligned16(const Tensor& t, const char* what) { TORCH_CHECK((reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0, what, ": 16-byte alignment needed"); }
+
+// One half (keys or values) of a paged 8-bit cache, codes given as bytes.
+struct Half {
+  void *codes, *scales;
+  int64_t blocks, nkv, block;
+};
+Half cache_half(const Tensor& codes, const Tensor& scales, const Tensor& with, const char* what) {
+  TORCH_CHECK(codes.dim() == 4 && codes.size(3) == 128, what, ": codes must be [blocks, kv_heads, block_size, 128]");
+  TORCH_CHECK(scales.dim() == 3 && scales.size(0) == codes.size(0) && scales.size(1) == codes.size(1) && scales.size(2) == codes.size(2), what,
+              ": scales must be [blocks, kv_heads, block_size]");
+  TORCH_CHECK(codes.size(0) >= 1 && codes.size(1) >= 1, what, ": an empty cache");
+  same_device(codes, with, what);
+  same_device(scales, with, what);
+  Half h{data(codes, U8, 1, what), data(scales, U8, 1, what), codes.size(0), codes.size(1), codes.size(2)};
+  aligned16(codes, what);
+  aligned16(scales, what);
+  TORCH_CHECK(h.block >= 16 && (h.block & (h.block - 1)) == 0, what, ": block_size must be a power of two from 16 on");
+  TORCH_CHECK(h.blocks * h.nkv * h.block <= INT32_MAX, what, ": more than 2^31 - 1 token rows");
+  return h;
+}
+
+const void* norm_weight(const OptTensor& w, const Tensor& with, const char* what) {
+  if (!w.has_value()) return nullptr;
+  TORCH_CHECK(w->numel() == 128, what, ": norm weights have 128 entries");
+  same_device(*w, with, what);
+  return data(*w, BF, 128, what);
+}
+
+void fp8_store(const Tensor& qkv, const OptTensor& qw, const OptTensor& kw, double eps, const OptTensor& rope, const Tensor& positions,
+               const Tensor& slots, Tensor& q_out, const Tensor& k_codes, const Tensor& k_scales, const Tensor& v_codes, const Tensor& v_scales,
+               int64_t nq, const Tensor& status) {
+  const Half k = cache_half(k_codes, k_scales, qkv, "fp8_store"), v = cache_half(v_codes, v_scales, qkv, "fp8_store");
+  TORCH_CHECK(k_codes.sizes() == v_codes.sizes(), "fp8_store: keys and values of one shape expected");
+  TORCH_CHECK(qkv.dim() == 2 && nq >= 1, "fp8_store: qkv must be [T, (nq + 2 nkv) * 128]");
+  const int64_t T = qkv.size(0);
+  view2(qkv, BF, T, (nq + 2 * k.nkv) * 128, "fp8_store: qkv");
+  TORCH_CHECK(T <= 1 || qkv.stride(0) >= qkv.size(1), "fp8_store: rows of qkv overlap");
+  const float* rp = nullptr;
+  int rope_rows = 0;
+  if (rope.has_value()) {
+    TORCH_CHECK(rope->dim() == 2 && rope->size(1) == 128 && rope->size(0) >= 1, "fp8_store: the rotation table must be [positions, 128]");
+    same_device(*rope, qkv, "fp8_store");
+    rp = floats(*rope, 128, "fp8_store: rotation table");
+    aligned16(*rope, "fp8_store: rotation table");
+    rope_rows = i32(rope->size(0));
+  }
+  same_device(positions, qkv, "fp8_store");
+  same_device(slots, qkv, "fp8_store");
+  same_device(q_out, qkv, "fp8_store");
+  same_device(status, qkv, "fp8_store");
+  TORCH_CHECK(q_out.numel() == T * nq * 128, "fp8_store: q must have T * nq * 128 entries");
+  void* qp = data(q_out, BF, 0, "fp8_store: q");
+  if (T > 0) aligned16(q_out, "fp8_store: q");
+  const c10::cuda::CUDAGuard guard(qkv.device());
+  check_rc(forge_fp8_store(qkv.data_ptr(), T > 1 ? qkv.stride(0) : qkv.size(1), norm_weight(qw, qkv, "fp8_store"), norm_weight(kw, qkv, "fp8_store"),
+                           static_cast<float>(eps), rp, rope_rows, ints(positions, T, "fp8_store: positions"), ints(slots, T, "fp8_store: slots"), qp,
+                           k.codes, k.scales, v.codes, v.scales, i32(T), i32(nq), i32(k.nkv), i32(k.block), k.blocks * k.block,
+                           status_word(status), stream_of(qkv)),
+           "forge_fp8_store");
+}
+
+void fp8_expand(const Tensor& k_codes, const Tensor& k_scales, const Tensor& v_codes, const Tensor& v_scales, const Tensor& block_tables,
+                const Tensor& lens, Tensor& k_out, Tensor& v_out, Tensor& tables, const Tensor& status) {
+  const Half k = cache_half(k_codes, k_scales, k_codes, "fp8_expand"), v = cache_half(v_codes, v_scales, k_codes, "fp8_expand");
+  TORCH_CHECK(k_codes.sizes() == v_codes.sizes(), "fp8_expand: keys and values of one shape expected");
+  TORCH_CHECK(block_tables.dim() == 2 && tables.sizes() == block_tables.sizes(), "fp8_expand: tables must be [sequences, width]");
+  TORCH_CHECK(k_out.dim() == 4 && k_out.size(1) == k.nkv && k_out.size(2) == k.block && k_out.size(3) == 128 && v_out.sizes() == k_out.sizes(),
+              "fp8_expand: pages must be [capacity, kv_heads, block_size, 128]");
+  for (const Tensor* t : std::initializer_list<const Tensor*>{&block_tables, &lens, &k_out, &v_out, &tables, &status}) same_device(*t, k_codes, "fp8_expand");
+  const int64_t S = block_tables.size(0), W = block_tables.size(1);
+  TORCH_CHECK(S <= 65535 && W * k.block <= INT32_MAX, "fp8_expand: too many sequences or too wide a table");
+  void *kp = data(k_out, BF, 0, "fp8_expand: keys"), *vp = data(v_out, BF, 0, "fp8_expand: values");
+  if (k_out.numel() > 0) {
+    aligned16(k_out, "fp8_expand: keys");
+    aligned16(v_out, "fp8_expand: values");
+  }
+  const c10::cuda::CUDAGuard guard(k_codes.device());
+  check_rc(forge_fp8_expand(k.codes, k.scales, v.codes, v.scales, ints(block_tables, S * W, "fp8_expand: tables"), ints(lens, S, "fp8_expand: lengths"),
+                            i32(S), i32(W), i32(k.blocks), i32(k.nkv), i32(k.block), kp, vp, const_cast<int*>(ints(tables, S * W, "fp8_expand: tables")),
+                            i32(k_out.size(0)), status_word(status), stream_of(k_codes)),
+           "forge_fp8_expand");
+}
+
+void decode_fp8(const Tensor& q, const Tensor& k_codes, const Tensor& k_scales, const Tensor& v_codes, const Tensor& v_scales,
+                const Tensor& block_tables, const Tensor& lens, Tensor& out, double scale, const Tensor& status) {
+  const Half k = cache_half(k_codes, k_scales, q, "decode_fp8"), v = cache_half(v_codes, v_scales, q, "decode_fp8");
+  TORCH_CHECK(k_codes.sizes() == v_codes.sizes(), "decode_fp8: keys and values of one shape expected");
+  TORCH_CHECK(q.dim() == 3 && q.size(2) == 128 && block_tables.dim() == 2, "decode_fp8: q must be [sequences, heads, 128], tables [sequences, width]");
+  const int64_t B = q.size(0), nq = q.size(1), W = block_tables.size(1);
+  TORCH_CHECK(nq >= 1 && nq % k.nkv == 0, "decode_fp8: query heads must be a multiple of the KV heads");
+  TORCH_CHECK(block_tables.size(0) >= B && out.numel() == B * nq * 128, "decode_fp8: shape mismatch");
+  TORCH_CHECK(W * k.block <= INT32_MAX, "decode_fp8: too wide a table");
+  for (const Tensor* t : std::initializer_list<const Tensor*>{&block_tables, &lens, &out, &status}) same_device(*t, q, "decode_fp8");
+  const void* qp = data(q, BF, 0, "decode_fp8: q");
+  void* op = data(out, BF, 0, "decode_fp8: out");
+  if (B > 0) {
+    aligned16(q, "decode_fp8: q");
+    aligned16(out, "decode_fp8: out");
+  }
+  const c10::cuda::CUDAGuard guard(q.device());
+  check_rc(forge_decode_fp8(qp, k.codes, k.scales, v.codes, v.scales, ints(block_tables, B * W, "decode_fp8: tables"), ints(lens, B, "decode_fp8: lengths"),
+                            op, i32(B), i32(nq), i32(k.nkv), i32(k.block), i32(W), i32(k.blocks), static_cast<float>(scale), status_word(status),
+                            stream_of(q)),
+           "forge_decode_fp8");
+}
+
+void rms_norm_fp8(const Tensor& x, const OptTensor& residual, const Tensor& w, Tensor& codes, Tensor& scales, double eps) {
+  TORCH_CHECK(x.dim() == 2 && x.size(1) >= 128 && x.size(1) % 128 == 0 && x.size(1) <= 16384,
+              "rms_norm_fp8: rows must have a multiple of 128 entries, at most 16384");
+  const int64_t M = x.size(0), H = x.size(1);
+  TORCH_CHECK(w.numel() == H && codes.numel() == M * H, "rms_norm_fp8: shape mismatch");
+  TORCH_CHECK(scales.dim() == 2 && scales.size(0) == H / 128 && scales.size(1) >= M, "rms_norm_fp8: scales must be [H / 128, >= rows]");
+  void* res = nullptr;
+  if (residual.has_value()) {
+    TORCH_CHECK(residual->sizes() == x.sizes(), "rms_norm_fp8: residual of the shape of x expected");
+    same_device(*residual, x, "rms_norm_fp8");
+    res = data(*residual, BF, 0, "rms_norm_fp8: residual");
+    if (M > 0) aligned16(*residual, "rms_norm_fp8: residual");
+  }
+  for (const Tensor* t : std::initializer_list<const Tensor*>{&w, &codes, &scales}) same_device(*t, x, "rms_norm_fp8");
+  const void *xp = data(x, BF, 0, "rms_norm_fp8: x"), *wp = data(w, BF, H, "rms_norm_fp8: weight");
+  void* cp = data(codes, U8, 0, "rms_norm_fp8: codes");
+  if (M > 0) {
+    aligned16(x, "rms_norm_fp8: x");
+    aligned16(w, "rms_norm_fp8: weight");
+    aligned16(codes, "rms_norm_fp8: codes");
+  }
+  const c10::cuda::CUDAGuard guard(x.device());
+  check_rc(forge_rms_norm_fp8(xp, res, wp, cp, floats(scales, 0, "rms_norm_fp8: scales"), i32(scales.size(1)), i32(M), i32(H),
+                              static_cast<float>(eps), stream_of(x)),
+           "forge_rms_norm_fp8");
+}
+
+}  // namespace
+
+void register_fp8(pybind11::module& m) {
+  m.def("fp8_store", &fp8_store);
+  m.def("fp8_expand", &fp8_expand);
+  m.def("decode_fp8", &decode_fp8);
+  m.def("rms_norm_fp8", &rms_norm_fp8);
+}

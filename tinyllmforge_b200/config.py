@@ -10,7 +10,7 @@ keyword arguments of ``LLM``).  Differences, all deliberate:
 * ``config.json`` is parsed directly into :class:`ModelConfig`, so building an
   engine does not import ``transformers``;
 * extra optional fields: ``seed``, ``dtype``, ``device``, ``comm``,
-  ``quantization``, ``load_format``, ``skip_tokenizer_init``, ``chunked_prefill``.
+  ``quantization``, ``kv_cache_dtype``, ``load_format``, ``skip_tokenizer_init``, ``chunked_prefill``.
 """
 from __future__ import annotations
 
@@ -124,6 +124,7 @@ class ModelConfig:
     def dtype(self) -> torch.dtype:
         return parse_dtype(self.torch_dtype)
 
+    cache_quantizable = True         # keys and values may be held in 8 bits
     prefix_cacheable = True          # every block of the KV cache is a function of the tokens before it alone
     num_recurrent_runs = 0           # layer runs that keep a per-sequence state beside the paged cache
 
@@ -174,6 +175,7 @@ class Config:
     device: str = "auto"                     # "auto" | "cuda" | "cpu"
     comm: str = "fused"                      # "fused": in-kernel NVLink collectives; "nccl": torch.distributed calls
     quantization: Optional[str] = None       # None | "fp8_block"
+    kv_cache_dtype: Optional[str] = None     # None: the model's type | "fp8": e4m3 with a power-of-two scale per token and head
     load_format: str = "auto"                # "auto": read *.safetensors; "dummy": seeded N(0, 0.02) weights
     skip_tokenizer_init: bool = False
     rpc_timeout_s: float = 120.0             # bound on every control-plane wait between ranks
@@ -215,11 +217,18 @@ class Config:
             raise ValueError("comm must be 'fused' or 'nccl'")
         if self.quantization not in (None, "fp8_block"):
             raise ValueError("quantization must be None or 'fp8_block'")
+        if self.kv_cache_dtype not in (None, "fp8"):
+            raise ValueError("kv_cache_dtype must be None or 'fp8'")
         if self.load_format not in ("auto", "dummy"):
             raise ValueError("load_format must be 'auto' or 'dummy'")
         if self.quantization is not None and not getattr(hf, "quantizable", True):
             raise ValueError(f"quantization={self.quantization!r} is not available for {type(hf).__name__}")
         self.dtype = parse_dtype(self.dtype) if self.dtype is not None else hf.dtype
+        if self.kv_cache_dtype is not None:
+            if not getattr(hf, "cache_quantizable", False):
+                raise ValueError(f"kv_cache_dtype={self.kv_cache_dtype!r} is not available for {type(hf).__name__}")
+            if self.device == "cuda" and (hf.head_dim != 128 or self.dtype != torch.bfloat16):
+                raise ValueError(f"kv_cache_dtype={self.kv_cache_dtype!r} on the GPU needs heads of 128 entries and a bfloat16 model, got {hf.head_dim} and {self.dtype}")
         if self.eos < 0 and hf.eos_token_id is not None:
             self.eos = hf.eos_token_id
 

@@ -40,6 +40,7 @@ class DeviceBatch:
         self.max_seqlen_q, self.max_seqlen_k = sb.max_seqlen_q, sb.max_seqlen_k
         self.num_single, self.kv_rows = sb.num_single, sb.kv_rows
         self.step_index, self.seed = sb.step_index, sb.seed
+        self.key_lens = sb.section("context_lens")[:sb.num_seqs].tolist() if sb.is_prefill else None
         self.words = words
         self.header = words[:HEADER_WORDS]
         for name in SECTIONS:

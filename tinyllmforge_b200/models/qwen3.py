@@ -25,6 +25,7 @@ import torch
 
 from ..config import ModelConfig
 from ..ops import ref as ref_ops
+from ..ops.quant import Fp8BlockWeight, Fp8KVCache
 from ..parallel.comm import TPGroup
 from ..parallel.tp_layers import (MergedColumnParallelLinear, ParallelLMHead, QKVParallelLinear,
                                   RowParallelLinear, VocabParallelEmbedding)
@@ -75,8 +76,10 @@ class Qwen3ForCausalLM:
             self.lm_head.weight = self.embed_tokens.weight
         self.rope = ref_ops.rope_table(max_positions or cfg.max_position_embeddings, cfg.head_dim, cfg.rope_theta,
                                        self.device)
-        self.kv_cache: torch.Tensor | None = None      # [L, 2, blocks, kv_heads, block_size, d]
+        self.kv_cache: torch.Tensor | Fp8KVCache | None = None      # [L, 2, blocks, kv_heads, block_size, d]
+        self.fp8_cache = False                         # keys and values in 8 bits
         self.norms_folded = False                      # see fold_norm_weights()
+        self.norms_fp8 = False                         # see _forward_fp8()
 
     # ------------------------------------------------------------------ parameters by Hugging Face name
     def named_parameters(self):
@@ -109,36 +112,44 @@ class Qwen3ForCausalLM:
 
     # ------------------------------------------------------------------ cache
     def kv_block_bytes(self, block_size: int) -> int:
-        return 2 * len(self.layers) * block_size * self.num_kv_heads * self.head_dim * self.norm.element_size()
+        head_bytes = self.head_dim + 1 if self.fp8_cache else self.head_dim * self.norm.element_size()
+        return 2 * len(self.layers) * block_size * self.num_kv_heads * head_bytes
 
     def state_bytes(self) -> int:
         """Per-sequence state beside the paged cache: none."""
         return 0
 
     def expansion_bytes(self, tokens: int) -> int:
-        return 0
+        """Workspace of ``tokens`` cached keys that a prompt's attention reads back from 8 bits."""
+        return 2 * tokens * self.num_kv_heads * self.head_dim * self.norm.element_size() if self.fp8_cache else 0
 
     def bind_cache(self, num_blocks: int, block_size: int, num_slots: int = 0) -> None:
+        if self.fp8_cache:
+            self.bind_kv_cache(Fp8KVCache.zeros(len(self.layers), 2, num_blocks, self.num_kv_heads, block_size, self.head_dim, device=self.device))
+            return
         self.bind_kv_cache(torch.zeros(len(self.layers), 2, num_blocks, self.num_kv_heads, block_size, self.head_dim, dtype=self.dtype,
                                        device=self.device))
 
     def drop_cache(self) -> None:
         self.kv_cache = None
 
-    def bind_kv_cache(self, kv_cache: torch.Tensor) -> None:
+    def bind_kv_cache(self, kv_cache: torch.Tensor | Fp8KVCache) -> None:
         assert kv_cache.shape[0] == len(self.layers) and kv_cache.shape[1] == 2
         self.kv_cache = kv_cache
+        self.fp8_cache = isinstance(kv_cache, Fp8KVCache)
 
     def finish_loading(self, config) -> None:
-        """What follows loading: norm folding (single GPU, bf16) or block-wise fp8 quantisation of the four projections."""
+        """What follows loading: the cache's type, norm folding (single GPU, bf16) or block-wise fp8 quantisation of the four
+        projections.  With both in 8 bits the norms hand 8-bit rows to the projections (``_forward_fp8``)."""
+        self.fp8_cache = config.kv_cache_dtype == "fp8"
         if (config.device == "cuda" and self.tp.size == 1 and config.quantization is None and config.dtype == torch.bfloat16
                 and config.extra.get("fold_norms", True) and not self.cfg.attention_bias):
             self.fold_norm_weights()            # add + RMSNorm become GEMM epilogues
         if config.quantization == "fp8_block":
-            from ..ops.quant import Fp8BlockWeight
             for l in self.layers:               # embeddings and LM head stay bf16
                 for lin in (l.qkv_proj, l.o_proj, l.gate_up_proj, l.down_proj):
                     lin.weight = Fp8BlockWeight.quantize(lin.weight)
+            self.norms_fp8 = self.fp8_cache and self.tp.size == 1
 
     # ------------------------------------------------------------------ norm folding (single GPU, CUDA op set)
     def fold_norm_weights(self) -> None:
@@ -161,8 +172,8 @@ class Qwen3ForCausalLM:
         squares from the GEMM that updates the residual stream to the GEMM that reads it."""
         ops, layers = self.ops, self.layers
         residual, ssq_a, ssq_b = ops.embedding_ssq(batch.input_ids, self.embed_tokens.weight, self.embed_tokens.vocab_start)
-        fused_decode = (not batch.is_prefill and self.head_dim == 128 and batch.padded_seqs <= ops.fused_qkv_max_batch)
-        in_gemm = ops.qkv_rope_store_in_gemm(residual.shape[0], self.head_dim, layers[0].qkv_proj.weight, batch.is_prefill)
+        fused_decode = (not batch.is_prefill and self.head_dim == 128 and batch.padded_seqs <= ops.fused_qkv_max_batch and not self.fp8_cache)
+        in_gemm = not self.fp8_cache and ops.qkv_rope_store_in_gemm(residual.shape[0], self.head_dim, layers[0].qkv_proj.weight, batch.is_prefill)
         for i, l in enumerate(layers):
             kc, vc = self.kv_cache[i, 0], self.kv_cache[i, 1]
             if in_gemm:         # norm, rotation and cache write in the projection's epilogue: one launch less per block
@@ -182,6 +193,22 @@ class Qwen3ForCausalLM:
             ops.linear_residual(g, l.down_proj.weight, residual, ssq_a)
         return ops.rms_norm(residual, self.norm, self.eps)
 
+    # ------------------------------------------------------------------ weights and cache in 8 bits (single GPU)
+    def _forward_fp8(self, batch) -> torch.Tensor:
+        """The block loop with block-scaled fp8 weights and an 8-bit cache: the norms hand 8-bit rows to qkv_proj and gate_up_proj, so
+        that these need no quantiser launch of their own (two less per block)."""
+        ops, residual = self.ops, None
+        x = ops.embedding(batch.input_ids, self.embed_tokens.weight, self.embed_tokens.vocab_start)
+        for i, l in enumerate(self.layers):
+            kc, vc = self.kv_cache[i, 0], self.kv_cache[i, 1]
+            h, residual = ops.rms_norm_fp8(x, residual, l.input_layernorm, self.eps)
+            q = ops.qk_norm_rope_store(l.qkv_proj.forward(ops, h), l.q_norm, l.k_norm, self.eps, self.rope, batch.positions,
+                                       batch.slot_mapping, kc, vc, self.num_heads, self.num_kv_heads, self.head_dim)
+            x = l.o_proj.forward(ops, ops.attention(q, kc, vc, batch, self.scale))
+            h, residual = ops.rms_norm_fp8(x, residual, l.post_attention_layernorm, self.eps)
+            x = l.down_proj.forward(ops, l.gate_up_proj.forward_silu_mul(ops, h))
+        return ops.add_rms_norm(x, residual, self.norm, self.eps)[0]
+
     # ------------------------------------------------------------------ forward
     def forward(self, batch) -> torch.Tensor:
         """Hidden states ``[tokens, hidden]`` after the final norm.
@@ -193,13 +220,16 @@ class Qwen3ForCausalLM:
         if self.norms_folded:
             return self._forward_folded(batch)
         ops = self.ops
+        if self.norms_fp8 and all(ops.takes_fp8_rows(lin.weight, batch.input_ids.shape[0])
+                                  for lin in (self.layers[0].qkv_proj, self.layers[0].gate_up_proj)):
+            return self._forward_fp8(batch)
         layers = self.layers
         x, residual = ops.embed_norm(batch.input_ids, self.embed_tokens, layers[0].input_layernorm, self.eps)
         # small decode steps on the GPU: q/k-norm + rotation + KV store run inside the attention kernel (one launch less per
         # layer; at large batches the attention kernel is bandwidth-bound and the extra work per sequence costs more)
-        fused_decode = (not batch.is_prefill and self.head_dim == 128 and hasattr(ops, "decode_attention_qkv")
+        fused_decode = (not batch.is_prefill and self.head_dim == 128 and hasattr(ops, "decode_attention_qkv") and not self.fp8_cache
                         and batch.padded_seqs <= ops.fused_qkv_max_batch)
-        in_gemm = (hasattr(ops, "qkv_rope_store_in_gemm") and getattr(layers[0].qkv_proj, "bias", None) is None
+        in_gemm = (hasattr(ops, "qkv_rope_store_in_gemm") and not self.fp8_cache and getattr(layers[0].qkv_proj, "bias", None) is None
                    and ops.qkv_rope_store_in_gemm(x.shape[0], self.head_dim, layers[0].qkv_proj.weight, batch.is_prefill))
         for i, l in enumerate(layers):
             kc, vc = self.kv_cache[i, 0], self.kv_cache[i, 1]

@@ -17,9 +17,10 @@ import torch
 
 from ..config import Config
 from ..parallel.comm import TPGroup
+from .cuda_fp8 import Fp8Ops
 from .cuda_hybrid import HybridOps
 from .cuda_mixers import MixerOps
-from .quant import Fp8BlockWeight
+from .quant import Fp8BlockWeight, Fp8KVCache, Fp8Rows
 
 try:
     from .. import _C
@@ -85,7 +86,7 @@ def _streamk_workspace(C, device, num_sms: int) -> None:
     _STREAMK_WS[key] = (ws, counters)
 
 
-class CudaOps(MixerOps, HybridOps):
+class CudaOps(MixerOps, HybridOps, Fp8Ops):
     name = "cuda"
 
     def __init__(self, config: Config | None = None, tp: TPGroup | None = None, device=None):
@@ -119,6 +120,7 @@ class CudaOps(MixerOps, HybridOps):
         self.fp8_expand_max_weights = int(os.environ.get("FORGE_FP8_EXPAND_MAX_WEIGHTS", "0"))
         self._fp8_scratch = None                   # bf16 expansion of one fp8 weight (see _expand_fp8)
         self._fp8_retired = []
+        self.expand_tokens = config.max_num_batched_tokens if config is not None else 16384   # see prefill_attention_fp8
 
     @property
     def launches(self) -> int:
@@ -149,7 +151,7 @@ class CudaOps(MixerOps, HybridOps):
         """x @ w.T.  ``w`` must not be the output of the kernel launched just before this call: the decode
         kernel starts streaming weights before it waits for its predecessor (weights are static in the engine)."""
         if isinstance(w, Fp8BlockWeight):
-            if not self._expands_fp8(w, x.shape[0]):
+            if isinstance(x, Fp8Rows) or not self._expands_fp8(w, x.shape[0]):
                 return self.linear_fp8(x, w)
             w, force_deep = self._expand_fp8(w), force_deep | W_DYNAMIC
         if not self.tma_ok(x, w):
@@ -161,7 +163,7 @@ class CudaOps(MixerOps, HybridOps):
     def linear_silu_mul(self, x: torch.Tensor, w_gate_up: torch.Tensor, force_mode: int = 0, force_splits: int = 0,
                         force_block_c: int = 0, force_deep: int = 0) -> torch.Tensor:
         if isinstance(w_gate_up, Fp8BlockWeight):
-            if not self._expands_fp8(w_gate_up, x.shape[0]):
+            if isinstance(x, Fp8Rows) or not self._expands_fp8(w_gate_up, x.shape[0]):
                 return self.silu_mul(self.linear_fp8(x, w_gate_up))
             w_gate_up, force_deep = self._expand_fp8(w_gate_up), force_deep | W_DYNAMIC
         if not self.tma_ok(x, w_gate_up):
@@ -218,12 +220,15 @@ class CudaOps(MixerOps, HybridOps):
         return out
 
     def linear_fp8(self, x: torch.Tensor, w: "Fp8BlockWeight") -> torch.Tensor:
-        """Block-scaled fp8 GEMM: quantise activations per token and 128 features, multiply on the e4m3 tensor-core
+        """Block-scaled fp8 GEMM: quantise activations per token and 128 features (``Fp8Rows`` are), multiply on the e4m3 tensor-core
         path, apply the scales per K block while accumulating."""
         M, K = x.shape
-        xq = torch.empty(M, K, dtype=torch.uint8, device=x.device)
-        xs = torch.empty(K // 128, (M + 3) // 4 * 4, dtype=torch.float32, device=x.device)
-        self.C.quant_fp8(x, xq, xs)
+        if isinstance(x, Fp8Rows):
+            xq, xs = x.q.view(torch.uint8), x.scale
+        else:
+            xq = torch.empty(M, K, dtype=torch.uint8, device=x.device)
+            xs = torch.empty(K // 128, (M + 3) // 4 * 4, dtype=torch.float32, device=x.device)
+            self.C.quant_fp8(x, xq, xs)
         N = w.shape[0]
         out = torch.empty(M, N, dtype=x.dtype, device=x.device)
         splits = self.C.gemm_fp8_splits(M, N, K)         # few tokens: K is split over CTAs, partials added by a second kernel
@@ -263,6 +268,10 @@ class CudaOps(MixerOps, HybridOps):
 
     def qk_norm_rope_store(self, qkv, q_weight, k_weight, eps, table, positions, slot_mapping, k_cache, v_cache,
                            num_heads, num_kv_heads, head_dim, do_rope=True):
+        if isinstance(k_cache, Fp8KVCache):
+            if (num_kv_heads, head_dim) != (k_cache.shape[1], k_cache.shape[3]):
+                raise ValueError(f"{num_kv_heads} KV heads of {head_dim} entries do not fit a cache of shape {tuple(k_cache.shape)}")
+            return self.store_fp8(qkv, q_weight, k_weight, eps, table, positions, slot_mapping, k_cache, v_cache, num_heads, do_rope)
         T = qkv.shape[0]
         q = torch.empty(T, num_heads, head_dim, dtype=qkv.dtype, device=qkv.device)
         self.C.qk_norm_rope_store(qkv, q_weight, k_weight, eps, table, positions, slot_mapping, q, k_cache, v_cache,
@@ -300,6 +309,8 @@ class CudaOps(MixerOps, HybridOps):
 
     # ------------------------------------------------------------------ attention
     def attention(self, q, k_cache, v_cache, batch, scale):
+        if isinstance(k_cache, Fp8KVCache):
+            return (self.prefill_attention_fp8 if batch.is_prefill else self.decode_attention_fp8)(q, k_cache, v_cache, batch, scale)
         T, H, D = q.shape
         out = torch.empty(T, H * D, dtype=q.dtype, device=q.device)
         if batch.is_prefill:

@@ -1,0 +1,80 @@
+"""CUDA ops that keep keys, values and normed rows in 8 bits (types: ``ops/quant.py``).
+
+Queries and results are bf16, heads have 128 entries, cache blocks 16 tokens or more (a power of two).
+"""
+from __future__ import annotations
+
+import torch
+
+from .quant import BLOCK, Fp8KVCache, Fp8Rows
+
+
+class Fp8Ops:
+    """Mixed into ``CudaOps`` (uses its ``C``, ``status``, ``device`` and ``num_sms``)."""
+
+    @staticmethod
+    def _halves(k_cache, v_cache) -> tuple:
+        if not (isinstance(k_cache, Fp8KVCache) and isinstance(v_cache, Fp8KVCache)):
+            raise TypeError("keys and values must both be held in 8 bits, or neither")
+        return k_cache.code_bytes, k_cache.scales, v_cache.code_bytes, v_cache.scales
+
+    def store_fp8(self, qkv, q_weight, k_weight, eps, table, positions, slot_mapping, k_cache, v_cache, num_heads, do_rope=True):
+        """``qk_norm_rope_store`` into an 8-bit cache: what is stored is rounded once, from fp32, and so is q.  The slots of a call are
+        distinct; a negative one is passed over."""
+        q = torch.empty(qkv.shape[0], num_heads, 128, dtype=qkv.dtype, device=qkv.device)
+        self.C.fp8_store(qkv, q_weight, k_weight, eps, table if do_rope else None, positions, slot_mapping, q, *self._halves(k_cache, v_cache),
+                         num_heads, self.status)
+        return q
+
+    def expand_kv(self, k_cache, v_cache, block_tables, context_lens, num_pages):
+        """The sequences' pages read back, in order: (keys, values) bf16 ``[num_pages, kv_heads, block_size, 128]``, exact, entries behind a
+        sequence's last token zero; and the page numbers ``[sequences, width]``, -1 behind the last.  ``num_pages``: at least the
+        pages of all sequences (pages without a sequence are left as they are); one too many for it is reported and left out."""
+        halves = self._halves(k_cache, v_cache)
+        k, v = (torch.empty(num_pages, *k_cache.shape[1:], dtype=torch.bfloat16, device=k_cache.device) for _ in range(2))
+        tables = torch.empty_like(block_tables)
+        self.C.fp8_expand(*halves, block_tables, context_lens, k, v, tables, self.status)
+        return k, v, tables
+
+    def decode_attention_fp8(self, q, k_cache, v_cache, batch, scale):
+        out = torch.empty(q.shape[0], q.shape[1] * q.shape[2], dtype=q.dtype, device=q.device)
+        self.C.decode_fp8(q, *self._halves(k_cache, v_cache), batch.block_tables, batch.context_lens, out, scale, self.status)
+        return out
+
+    def prefill_attention_fp8(self, q, k_cache, v_cache, batch, scale):
+        """Prompts: the sequences' pages are read back and attended to by the bf16 kernels, as many sequences at a time as have
+        ``expand_pages`` pages together (one at least)."""
+        T, H, D = q.shape
+        out = torch.empty(T, H * D, dtype=q.dtype, device=q.device)
+        bs, lens = k_cache.shape[2], getattr(batch, "key_lens", None)
+        if lens is None:                          # lengths unknown on the host: as long as the table is wide
+            lens = [min(batch.max_seqlen_k, batch.block_tables.shape[1] * bs)] * batch.num_seqs
+        begin = 0
+        while begin < batch.num_seqs:
+            end, pages = begin, 0
+            while end < batch.num_seqs and (end == begin or pages + -(-lens[end] // bs) <= self.expand_pages(bs)):
+                pages += -(-lens[end] // bs)
+                end += 1
+            part = slice(begin, end)
+            k, v, tables = self.expand_kv(k_cache, v_cache, batch.block_tables[part], batch.context_lens[part], pages)
+            self.C.prefill_attention(q, k, v, batch.cu_seqlens_q[begin:end + 1], batch.context_lens[part], tables, out, end - begin,
+                                     batch.max_seqlen_q, scale, self.status)
+            begin = end
+        return out
+
+    def expand_pages(self, block_size: int) -> int:
+        return max(1, self.expand_tokens // block_size)
+
+    # ------------------------------------------------------------------ norms with 8-bit rows
+    def takes_fp8_rows(self, weight, rows: int) -> bool:
+        """Whether a projection with this weight multiplies 8-bit rows (with many rows fp8 weights are expanded and rows stay bf16)."""
+        return not isinstance(weight, torch.Tensor) and not self._expands_fp8(weight, rows)
+
+    def rms_norm_fp8(self, x, residual, weight, eps):
+        """(``Fp8Rows`` of the normed rows, residual): ``add_rms_norm`` whose normed rows leave in 8 bits, quantised from fp32 per 128 columns.
+        ``residual`` is updated in place and returned; without one x is."""
+        M, K = x.shape
+        q = torch.empty(M, K, dtype=torch.float8_e4m3fn, device=x.device)
+        scale = torch.empty(K // BLOCK, (M + 3) // 4 * 4, dtype=torch.float32, device=x.device)
+        self.C.rms_norm_fp8(x, residual, weight, q.view(torch.uint8), scale, eps)
+        return Fp8Rows(q, scale, x.dtype), x if residual is None else residual

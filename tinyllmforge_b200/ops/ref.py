@@ -24,7 +24,8 @@ import numpy as np
 import torch
 import torch.nn.functional as F
 
-from . import ref_hybrid
+from . import ref_fp8, ref_hybrid
+from .quant import Fp8KVCache
 
 
 # ----------------------------------------------------------------------------- norms
@@ -135,6 +136,9 @@ def qk_norm_rope_store(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torc
                        num_heads: int, num_kv_heads: int, head_dim: int) -> torch.Tensor:
     """Split the fused QKV projection, RMS-normalise q and k per head, rotate, write k and v into the
     paged cache and return q as ``[T, heads, d]`` (tinyvllm/models/qwen3.py:78-94)."""
+    if isinstance(k_cache, Fp8KVCache):
+        return ref_fp8.qk_norm_rope_store(qkv, q_weight, k_weight, eps, table, positions, slot_mapping, k_cache, v_cache, num_heads,
+                                          num_kv_heads, head_dim)
     T = qkv.shape[0]
     q, k, v = qkv.split([num_heads * head_dim, num_kv_heads * head_dim, num_kv_heads * head_dim], dim=-1)
     q = rms_norm(q.reshape(T, num_heads, head_dim), q_weight, eps)
@@ -150,6 +154,8 @@ def _gather_kv(cache: torch.Tensor, table_row: torch.Tensor, length: int) -> tor
     bs = cache.shape[2]
     nblk = (length + bs - 1) // bs
     blocks = cache[table_row[:nblk].long()]              # [nblk, kvh, bs, d]
+    if isinstance(cache, Fp8KVCache):
+        blocks = blocks.dequantize()
     kvh, d = blocks.shape[1], blocks.shape[3]
     return blocks.permute(1, 0, 2, 3).reshape(kvh, nblk * bs, d)[:, :length]
 
@@ -468,6 +474,8 @@ class RefOps(ref_hybrid.RefHybridOps):
     add_rms_norm = staticmethod(add_rms_norm)
     rms_norm = staticmethod(rms_norm)
     qk_norm_rope_store = staticmethod(qk_norm_rope_store)
+    expand_kv = staticmethod(ref_fp8.expand_kv)
+    rms_norm_fp8 = staticmethod(ref_fp8.rms_norm_fp8)
     stream_update = staticmethod(stream_update)
     stream_mix = staticmethod(stream_mix)
     latent_prepare = staticmethod(latent_prepare)
@@ -482,6 +490,10 @@ class RefOps(ref_hybrid.RefHybridOps):
     def attention(q, k_cache, v_cache, batch, scale):
         return attention(q, k_cache, v_cache, batch.cu_seqlens_q, batch.context_lens, batch.block_tables,
                          scale, batch.num_seqs)
+
+    @staticmethod
+    def takes_fp8_rows(weight, rows: int) -> bool:
+        return not isinstance(weight, torch.Tensor)
 
     @staticmethod
     def select_rows(x, index):
