@@ -16,8 +16,9 @@ int forge_fp8_expand(const void* k_codes, const void* k_scales, const void* v_co
                      const int* lens, int num_seqs, int table_width, int num_blocks, int nkv, int block_size, void* k_out, void* v_out,
                      int* tables, int capacity, unsigned* status, cudaStream_t stream);
 int forge_decode_fp8(const void* q, const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales,
-                     const int* block_tables, const int* lens, void* out, int B, int nq, int nkv, int block_size, int table_width,
+                     const int* block_tables, const int* lens, void* out, float* scratch, int B, int nq, int nkv, int block_size, int table_width,
                      int num_blocks, float scale, unsigned* status, cudaStream_t stream);
+long long forge_decode_fp8_scratch_floats(int B, int nq, int nkv, int block_size, int table_width);
 int forge_rms_norm_fp8(const void* x, void* residual, const void* w, void* codes, float* scales, int scale_ld, int rows, int H, float eps,
                        cudaStream_t stream);
 }
@@ -129,9 +130,10 @@ void decode_fp8(const Tensor& q, const Tensor& k_codes, const Tensor& k_scales, 
     aligned16(out, "decode_fp8: out");
   }
   const c10::cuda::CUDAGuard guard(q.device());
+  const Tensor scratch = at::empty({forge_decode_fp8_scratch_floats(i32(B), i32(nq), i32(k.nkv), i32(k.block), i32(W))}, q.options().dtype(at::kFloat));
   check_rc(forge_decode_fp8(qp, k.codes, k.scales, v.codes, v.scales, ints(block_tables, B * W, "decode_fp8: tables"), ints(lens, B, "decode_fp8: lengths"),
-                            op, i32(B), i32(nq), i32(k.nkv), i32(k.block), i32(W), i32(k.blocks), static_cast<float>(scale), status_word(status),
-                            stream_of(q)),
+                            op, scratch.data_ptr<float>(), i32(B), i32(nq), i32(k.nkv), i32(k.block), i32(W), i32(k.blocks), static_cast<float>(scale),
+                            status_word(status), stream_of(q)),
            "forge_decode_fp8");
 }
 

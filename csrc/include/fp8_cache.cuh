@@ -41,8 +41,9 @@ __device__ __forceinline__ uint32_t fp8_pack(float a, float b, float c, float d)
 }
 // Two codes (bits 0..15) -> two halves, exact.
 __device__ __forceinline__ uint32_t fp8_to_half2(uint32_t codes) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(codes), __NV_E4M3);
-  return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(codes)));
+  return h;
 }
 __device__ __forceinline__ float2 fp8_to_float2(uint32_t codes) {
   const uint32_t h = fp8_to_half2(codes & 0xFFFFu);

@@ -1,4 +1,4 @@
-// Warp-level bf16 products (mma.sync m16n8k16, fp32 accumulate), ldmatrix and 16-byte asynchronous copies: for products too
+// Warp-level bf16 and fp16 products (mma.sync m16n8k16, fp32 accumulate), ldmatrix and 16-byte asynchronous copies: for products too
 // small or too irregular for a 128-row UMMA tile.
 #pragma once
 
@@ -17,6 +17,19 @@ __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// The same with fp16 operands.  Lane l holds of a: rows l / 4 (a[0], a[2]) and l / 4 + 8 (a[1], a[3]), columns 2 (l % 4) + 0, 1 (a[0], a[1]) and eight
+// further on; of b: column l / 4, rows 2 (l % 4) + 0, 1 (b0) and eight further on (b1).
+__device__ __forceinline__ void mma16816_f16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Transpose of an 8 x 8 matrix of 16-bit values: lane l holds row l / 4, columns 2 (l % 4) + 0, 1, before and after.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 // 16 bytes global -> shared; `bytes` < 16 zero-fills the rest (0: nothing is read).
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
