@@ -5,6 +5,7 @@
 #include <torch/extension.h>
 
 #include <cstdint>
+#include <tuple>
 
 #include "checks.h"
 
@@ -27,11 +28,12 @@ namespace {
 
 constexpr auto BF = at::kBFloat16;
 constexpr auto U8 = at::kByte;
+constexpr auto E4M3 = at::kFloat8_e4m3fn;
 
 void same_device(const Tensor& a, const Tensor& b, const char* what) { TORCH_CHECK(a.device() == b.device(), what, ": tensors on one device expected"); }
 void aligned16(const Tensor& t, const char* what) { TORCH_CHECK((reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0, what, ": 16-byte alignment needed"); }
 
-// One half (keys or values) of a paged 8-bit cache, codes given as bytes.
+// One half (keys or values) of a paged 8-bit cache.
 struct Half {
   void *codes, *scales;
   int64_t blocks, nkv, block;
@@ -43,7 +45,7 @@ Half cache_half(const Tensor& codes, const Tensor& scales, const Tensor& with, c
   TORCH_CHECK(codes.size(0) >= 1 && codes.size(1) >= 1, what, ": an empty cache");
   same_device(codes, with, what);
   same_device(scales, with, what);
-  Half h{data(codes, U8, 1, what), data(scales, U8, 1, what), codes.size(0), codes.size(1), codes.size(2)};
+  Half h{data(codes, E4M3, 1, what), data(scales, U8, 1, what), codes.size(0), codes.size(1), codes.size(2)};
   aligned16(codes, what);
   aligned16(scales, what);
   TORCH_CHECK(h.block >= 16 && (h.block & (h.block - 1)) == 0, what, ": block_size must be a power of two from 16 on");
@@ -58,9 +60,10 @@ const void* norm_weight(const OptTensor& w, const Tensor& with, const char* what
   return data(*w, BF, 128, what);
 }
 
-void fp8_store(const Tensor& qkv, const OptTensor& qw, const OptTensor& kw, double eps, const OptTensor& rope, const Tensor& positions,
-               const Tensor& slots, Tensor& q_out, const Tensor& k_codes, const Tensor& k_scales, const Tensor& v_codes, const Tensor& v_scales,
-               int64_t nq, const Tensor& status) {
+// Returns q [T, nq, 128].
+Tensor fp8_store(const Tensor& qkv, const OptTensor& qw, const OptTensor& kw, double eps, const OptTensor& rope, const Tensor& positions,
+                 const Tensor& slots, const Tensor& k_codes, const Tensor& k_scales, const Tensor& v_codes, const Tensor& v_scales, int64_t nq,
+                 const Tensor& status) {
   const Half k = cache_half(k_codes, k_scales, qkv, "fp8_store"), v = cache_half(v_codes, v_scales, qkv, "fp8_store");
   TORCH_CHECK(k_codes.sizes() == v_codes.sizes(), "fp8_store: keys and values of one shape expected");
   TORCH_CHECK(qkv.dim() == 2 && nq >= 1, "fp8_store: qkv must be [T, (nq + 2 nkv) * 128]");
@@ -78,71 +81,68 @@ void fp8_store(const Tensor& qkv, const OptTensor& qw, const OptTensor& kw, doub
   }
   same_device(positions, qkv, "fp8_store");
   same_device(slots, qkv, "fp8_store");
-  same_device(q_out, qkv, "fp8_store");
   same_device(status, qkv, "fp8_store");
-  TORCH_CHECK(q_out.numel() == T * nq * 128, "fp8_store: q must have T * nq * 128 entries");
-  void* qp = data(q_out, BF, 0, "fp8_store: q");
-  if (T > 0) aligned16(q_out, "fp8_store: q");
   const c10::cuda::CUDAGuard guard(qkv.device());
+  Tensor q = at::empty({T, nq, 128}, qkv.options());
   check_rc(forge_fp8_store(qkv.data_ptr(), T > 1 ? qkv.stride(0) : qkv.size(1), norm_weight(qw, qkv, "fp8_store"), norm_weight(kw, qkv, "fp8_store"),
-                           static_cast<float>(eps), rp, rope_rows, ints(positions, T, "fp8_store: positions"), ints(slots, T, "fp8_store: slots"), qp,
+                           static_cast<float>(eps), rp, rope_rows, ints(positions, T, "fp8_store: positions"), ints(slots, T, "fp8_store: slots"), q.data_ptr(),
                            k.codes, k.scales, v.codes, v.scales, i32(T), i32(nq), i32(k.nkv), i32(k.block), k.blocks * k.block,
                            status_word(status), stream_of(qkv)),
            "forge_fp8_store");
+  return q;
 }
 
-void fp8_expand(const Tensor& k_codes, const Tensor& k_scales, const Tensor& v_codes, const Tensor& v_scales, const Tensor& block_tables,
-                const Tensor& lens, Tensor& k_out, Tensor& v_out, Tensor& tables, const Tensor& status) {
+// Returns (keys, values) [pages, nkv, block_size, 128] and the page numbers [sequences, width].
+std::tuple<Tensor, Tensor, Tensor> fp8_expand(const Tensor& k_codes, const Tensor& k_scales, const Tensor& v_codes, const Tensor& v_scales,
+                                              const Tensor& block_tables, const Tensor& lens, int64_t pages, const Tensor& status) {
   const Half k = cache_half(k_codes, k_scales, k_codes, "fp8_expand"), v = cache_half(v_codes, v_scales, k_codes, "fp8_expand");
   TORCH_CHECK(k_codes.sizes() == v_codes.sizes(), "fp8_expand: keys and values of one shape expected");
-  TORCH_CHECK(block_tables.dim() == 2 && tables.sizes() == block_tables.sizes(), "fp8_expand: tables must be [sequences, width]");
-  TORCH_CHECK(k_out.dim() == 4 && k_out.size(1) == k.nkv && k_out.size(2) == k.block && k_out.size(3) == 128 && v_out.sizes() == k_out.sizes(),
-              "fp8_expand: pages must be [capacity, kv_heads, block_size, 128]");
-  for (const Tensor* t : std::initializer_list<const Tensor*>{&block_tables, &lens, &k_out, &v_out, &tables, &status}) same_device(*t, k_codes, "fp8_expand");
+  TORCH_CHECK(block_tables.dim() == 2 && pages >= 0, "fp8_expand: tables must be [sequences, width], and the pages not negative");
+  for (const Tensor* t : {&block_tables, &lens, &status}) same_device(*t, k_codes, "fp8_expand");
   const int64_t S = block_tables.size(0), W = block_tables.size(1);
   TORCH_CHECK(S <= 65535 && W * k.block <= INT32_MAX, "fp8_expand: too many sequences or too wide a table");
-  void *kp = data(k_out, BF, 0, "fp8_expand: keys"), *vp = data(v_out, BF, 0, "fp8_expand: values");
-  if (k_out.numel() > 0) {
-    aligned16(k_out, "fp8_expand: keys");
-    aligned16(v_out, "fp8_expand: values");
-  }
+  const int* bt = ints(block_tables, S * W, "fp8_expand: tables");
+  const int* ln = ints(lens, S, "fp8_expand: lengths");
   const c10::cuda::CUDAGuard guard(k_codes.device());
-  check_rc(forge_fp8_expand(k.codes, k.scales, v.codes, v.scales, ints(block_tables, S * W, "fp8_expand: tables"), ints(lens, S, "fp8_expand: lengths"),
-                            i32(S), i32(W), i32(k.blocks), i32(k.nkv), i32(k.block), kp, vp, const_cast<int*>(ints(tables, S * W, "fp8_expand: tables")),
-                            i32(k_out.size(0)), status_word(status), stream_of(k_codes)),
+  const auto bf16 = k_codes.options().dtype(BF);
+  Tensor k_out = at::empty({pages, k.nkv, k.block, 128}, bf16), v_out = at::empty({pages, k.nkv, k.block, 128}, bf16);
+  Tensor tables = at::empty({S, W}, block_tables.options());
+  check_rc(forge_fp8_expand(k.codes, k.scales, v.codes, v.scales, bt, ln, i32(S), i32(W), i32(k.blocks), i32(k.nkv), i32(k.block), k_out.data_ptr(),
+                            v_out.data_ptr(), tables.data_ptr<int>(), i32(pages), status_word(status), stream_of(k_codes)),
            "forge_fp8_expand");
+  return {k_out, v_out, tables};
 }
 
-void decode_fp8(const Tensor& q, const Tensor& k_codes, const Tensor& k_scales, const Tensor& v_codes, const Tensor& v_scales,
-                const Tensor& block_tables, const Tensor& lens, Tensor& out, double scale, const Tensor& status) {
+// Returns [sequences, nq * 128].
+Tensor decode_fp8(const Tensor& q, const Tensor& k_codes, const Tensor& k_scales, const Tensor& v_codes, const Tensor& v_scales,
+                  const Tensor& block_tables, const Tensor& lens, double scale, const Tensor& status) {
   const Half k = cache_half(k_codes, k_scales, q, "decode_fp8"), v = cache_half(v_codes, v_scales, q, "decode_fp8");
   TORCH_CHECK(k_codes.sizes() == v_codes.sizes(), "decode_fp8: keys and values of one shape expected");
   TORCH_CHECK(q.dim() == 3 && q.size(2) == 128 && block_tables.dim() == 2, "decode_fp8: q must be [sequences, heads, 128], tables [sequences, width]");
   const int64_t B = q.size(0), nq = q.size(1), W = block_tables.size(1);
   TORCH_CHECK(nq >= 1 && nq % k.nkv == 0, "decode_fp8: query heads must be a multiple of the KV heads");
-  TORCH_CHECK(block_tables.size(0) >= B && out.numel() == B * nq * 128, "decode_fp8: shape mismatch");
+  TORCH_CHECK(block_tables.size(0) >= B, "decode_fp8: a table for every sequence expected");
   TORCH_CHECK(W * k.block <= INT32_MAX, "decode_fp8: too wide a table");
-  for (const Tensor* t : std::initializer_list<const Tensor*>{&block_tables, &lens, &out, &status}) same_device(*t, q, "decode_fp8");
+  for (const Tensor* t : {&block_tables, &lens, &status}) same_device(*t, q, "decode_fp8");
   const void* qp = data(q, BF, 0, "decode_fp8: q");
-  void* op = data(out, BF, 0, "decode_fp8: out");
-  if (B > 0) {
-    aligned16(q, "decode_fp8: q");
-    aligned16(out, "decode_fp8: out");
-  }
+  if (B > 0) aligned16(q, "decode_fp8: q");
+  const int* bt = ints(block_tables, B * W, "decode_fp8: tables");
+  const int* ln = ints(lens, B, "decode_fp8: lengths");
   const c10::cuda::CUDAGuard guard(q.device());
+  Tensor out = at::empty({B, nq * 128}, q.options());
   const Tensor scratch = at::empty({forge_decode_fp8_scratch_floats(i32(B), i32(nq), i32(k.nkv), i32(k.block), i32(W))}, q.options().dtype(at::kFloat));
-  check_rc(forge_decode_fp8(qp, k.codes, k.scales, v.codes, v.scales, ints(block_tables, B * W, "decode_fp8: tables"), ints(lens, B, "decode_fp8: lengths"),
-                            op, scratch.data_ptr<float>(), i32(B), i32(nq), i32(k.nkv), i32(k.block), i32(W), i32(k.blocks), static_cast<float>(scale),
-                            status_word(status), stream_of(q)),
+  check_rc(forge_decode_fp8(qp, k.codes, k.scales, v.codes, v.scales, bt, ln, out.data_ptr(), scratch.data_ptr<float>(), i32(B), i32(nq), i32(k.nkv),
+                            i32(k.block), i32(W), i32(k.blocks), static_cast<float>(scale), status_word(status), stream_of(q)),
            "forge_decode_fp8");
+  return out;
 }
 
-void rms_norm_fp8(const Tensor& x, const OptTensor& residual, const Tensor& w, Tensor& codes, Tensor& scales, double eps) {
+// Returns the codes [rows, H] and their scales [H / 128, rows rounded up to 4].
+std::tuple<Tensor, Tensor> rms_norm_fp8(const Tensor& x, const OptTensor& residual, const Tensor& w, double eps) {
   TORCH_CHECK(x.dim() == 2 && x.size(1) >= 128 && x.size(1) % 128 == 0 && x.size(1) <= 16384,
               "rms_norm_fp8: rows must have a multiple of 128 entries, at most 16384");
   const int64_t M = x.size(0), H = x.size(1);
-  TORCH_CHECK(w.numel() == H && codes.numel() == M * H, "rms_norm_fp8: shape mismatch");
-  TORCH_CHECK(scales.dim() == 2 && scales.size(0) == H / 128 && scales.size(1) >= M, "rms_norm_fp8: scales must be [H / 128, >= rows]");
+  TORCH_CHECK(w.numel() == H, "rms_norm_fp8: a weight for every column expected");
   void* res = nullptr;
   if (residual.has_value()) {
     TORCH_CHECK(residual->sizes() == x.sizes(), "rms_norm_fp8: residual of the shape of x expected");
@@ -150,18 +150,16 @@ void rms_norm_fp8(const Tensor& x, const OptTensor& residual, const Tensor& w, T
     res = data(*residual, BF, 0, "rms_norm_fp8: residual");
     if (M > 0) aligned16(*residual, "rms_norm_fp8: residual");
   }
-  for (const Tensor* t : std::initializer_list<const Tensor*>{&w, &codes, &scales}) same_device(*t, x, "rms_norm_fp8");
+  same_device(w, x, "rms_norm_fp8");
   const void *xp = data(x, BF, 0, "rms_norm_fp8: x"), *wp = data(w, BF, H, "rms_norm_fp8: weight");
-  void* cp = data(codes, U8, 0, "rms_norm_fp8: codes");
-  if (M > 0) {
-    aligned16(x, "rms_norm_fp8: x");
-    aligned16(w, "rms_norm_fp8: weight");
-    aligned16(codes, "rms_norm_fp8: codes");
-  }
+  if (M > 0) aligned16(x, "rms_norm_fp8: x");
+  aligned16(w, "rms_norm_fp8: weight");
   const c10::cuda::CUDAGuard guard(x.device());
-  check_rc(forge_rms_norm_fp8(xp, res, wp, cp, floats(scales, 0, "rms_norm_fp8: scales"), i32(scales.size(1)), i32(M), i32(H),
-                              static_cast<float>(eps), stream_of(x)),
+  Tensor codes = at::empty({M, H}, x.options().dtype(E4M3)), scales = at::empty({H / 128, (M + 3) / 4 * 4}, x.options().dtype(at::kFloat));
+  check_rc(forge_rms_norm_fp8(xp, res, wp, codes.data_ptr(), scales.data_ptr<float>(), i32(scales.size(1)), i32(M), i32(H), static_cast<float>(eps),
+                              stream_of(x)),
            "forge_rms_norm_fp8");
+  return {codes, scales};
 }
 
 }  // namespace

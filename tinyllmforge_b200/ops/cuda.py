@@ -269,8 +269,9 @@ class CudaOps(MixerOps, HybridOps, Fp8Ops):
     def qk_norm_rope_store(self, qkv, q_weight, k_weight, eps, table, positions, slot_mapping, k_cache, v_cache,
                            num_heads, num_kv_heads, head_dim, do_rope=True):
         if isinstance(k_cache, Fp8KVCache):
-            if (num_kv_heads, head_dim) != (k_cache.shape[1], k_cache.shape[3]):
-                raise ValueError(f"{num_kv_heads} KV heads of {head_dim} entries do not fit a cache of shape {tuple(k_cache.shape)}")
+            shape = k_cache.shape
+            if num_kv_heads != shape[1] or head_dim != shape[3]:
+                raise ValueError(f"{num_kv_heads} KV heads of {head_dim} entries do not fit a cache of shape {tuple(shape)}")
             return self.store_fp8(qkv, q_weight, k_weight, eps, table, positions, slot_mapping, k_cache, v_cache, num_heads, do_rope)
         T = qkv.shape[0]
         q = torch.empty(T, num_heads, head_dim, dtype=qkv.dtype, device=qkv.device)

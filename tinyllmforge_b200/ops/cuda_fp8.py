@@ -6,7 +6,7 @@ from __future__ import annotations
 
 import torch
 
-from .quant import BLOCK, Fp8KVCache, Fp8Rows
+from .quant import Fp8KVCache, Fp8Rows
 
 
 class Fp8Ops:
@@ -16,30 +16,22 @@ class Fp8Ops:
     def _halves(k_cache, v_cache) -> tuple:
         if not (isinstance(k_cache, Fp8KVCache) and isinstance(v_cache, Fp8KVCache)):
             raise TypeError("keys and values must both be held in 8 bits, or neither")
-        return k_cache.code_bytes, k_cache.scales, v_cache.code_bytes, v_cache.scales
+        return k_cache.codes, k_cache.scales, v_cache.codes, v_cache.scales
 
     def store_fp8(self, qkv, q_weight, k_weight, eps, table, positions, slot_mapping, k_cache, v_cache, num_heads, do_rope=True):
         """``qk_norm_rope_store`` into an 8-bit cache: what is stored is rounded once, from fp32, and so is q.  The slots of a call are
         distinct; a negative one is passed over."""
-        q = torch.empty(qkv.shape[0], num_heads, 128, dtype=qkv.dtype, device=qkv.device)
-        self.C.fp8_store(qkv, q_weight, k_weight, eps, table if do_rope else None, positions, slot_mapping, q, *self._halves(k_cache, v_cache),
-                         num_heads, self.status)
-        return q
+        return self.C.fp8_store(qkv, q_weight, k_weight, eps, table if do_rope else None, positions, slot_mapping,
+                                *self._halves(k_cache, v_cache), num_heads, self.status)
 
     def expand_kv(self, k_cache, v_cache, block_tables, context_lens, num_pages):
         """The sequences' pages read back, in order: (keys, values) bf16 ``[num_pages, kv_heads, block_size, 128]``, exact, entries behind a
         sequence's last token zero; and the page numbers ``[sequences, width]``, -1 behind the last.  ``num_pages``: at least the
         pages of all sequences (pages without a sequence are left as they are); one too many for it is reported and left out."""
-        halves = self._halves(k_cache, v_cache)
-        k, v = (torch.empty(num_pages, *k_cache.shape[1:], dtype=torch.bfloat16, device=k_cache.device) for _ in range(2))
-        tables = torch.empty_like(block_tables)
-        self.C.fp8_expand(*halves, block_tables, context_lens, k, v, tables, self.status)
-        return k, v, tables
+        return self.C.fp8_expand(*self._halves(k_cache, v_cache), block_tables, context_lens, num_pages, self.status)
 
     def decode_attention_fp8(self, q, k_cache, v_cache, batch, scale):
-        out = torch.empty(q.shape[0], q.shape[1] * q.shape[2], dtype=q.dtype, device=q.device)
-        self.C.decode_fp8(q, *self._halves(k_cache, v_cache), batch.block_tables, batch.context_lens, out, scale, self.status)
-        return out
+        return self.C.decode_fp8(q, *self._halves(k_cache, v_cache), batch.block_tables, batch.context_lens, scale, self.status)
 
     def prefill_attention_fp8(self, q, k_cache, v_cache, batch, scale):
         """Prompts: the sequences' pages are read back and attended to by the bf16 kernels, as many sequences at a time as have
@@ -73,8 +65,5 @@ class Fp8Ops:
     def rms_norm_fp8(self, x, residual, weight, eps):
         """(``Fp8Rows`` of the normed rows, residual): ``add_rms_norm`` whose normed rows leave in 8 bits, quantised from fp32 per 128 columns.
         ``residual`` is updated in place and returned; without one x is."""
-        M, K = x.shape
-        q = torch.empty(M, K, dtype=torch.float8_e4m3fn, device=x.device)
-        scale = torch.empty(K // BLOCK, (M + 3) // 4 * 4, dtype=torch.float32, device=x.device)
-        self.C.rms_norm_fp8(x, residual, weight, q.view(torch.uint8), scale, eps)
+        q, scale = self.C.rms_norm_fp8(x, residual, weight, eps)
         return Fp8Rows(q, scale, x.dtype), x if residual is None else residual

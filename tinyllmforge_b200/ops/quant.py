@@ -59,13 +59,23 @@ class Fp8Rows:
     """Activations ``[M, K]`` as e4m3 values ``q`` with fp32 scales ``scale`` ``[K / 128, >= M]``, one per row and 128 columns: what a
     projection with an ``Fp8BlockWeight`` multiplies.  ``dtype``: the type of the projection's result."""
 
+    __slots__ = ("q", "scale", "dtype")
+
     def __init__(self, q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.bfloat16):
         if q.dtype != torch.float8_e4m3fn or scale.dtype != torch.float32 or q.dim() != 2 or scale.dim() != 2:
             raise ValueError("Fp8Rows: e4m3 values [M, K] and fp32 scales [K / 128, >= M] expected")
-        if q.shape[1] % BLOCK or scale.shape[0] != q.shape[1] // BLOCK or scale.shape[1] < q.shape[0]:
+        (M, K), (groups, columns) = q.shape, scale.shape
+        if K != groups * BLOCK or columns < M:
             raise ValueError(f"Fp8Rows: scales {tuple(scale.shape)} do not belong to values {tuple(q.shape)}")
         self.q, self.scale, self.dtype = q, scale, dtype
-        self.shape, self.device = tuple(q.shape), q.device
+
+    @property
+    def shape(self):
+        return self.q.shape
+
+    @property
+    def device(self):
+        return self.q.device
 
     def dequantize(self) -> torch.Tensor:
         M, K = self.shape
@@ -99,6 +109,8 @@ class Fp8KVCache:
     head (see ``quantize_heads``).  One layer's half is ``[blocks, kv_heads, block_size, head_dim]``, as the bf16 cache is; leading
     dimensions are indexed as a tensor's are, and the parts share the memory."""
 
+    __slots__ = ("codes", "scales")
+
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
         if codes.dtype != torch.float8_e4m3fn or scales.dtype != torch.uint8:
             raise ValueError(f"Fp8KVCache: float8_e4m3fn codes and uint8 scales expected, got {codes.dtype} and {scales.dtype}")
@@ -107,7 +119,18 @@ class Fp8KVCache:
         if codes.device != scales.device:
             raise ValueError("Fp8KVCache: codes and scales on one device expected")
         self.codes, self.scales = codes, scales
-        self.shape, self.dtype, self.device = codes.shape, codes.dtype, codes.device
+
+    @property
+    def shape(self):
+        return self.codes.shape
+
+    @property
+    def dtype(self):
+        return self.codes.dtype
+
+    @property
+    def device(self):
+        return self.codes.device
 
     @classmethod
     def zeros(cls, *shape: int, device="cpu") -> "Fp8KVCache":
