@@ -45,6 +45,14 @@ __device__ __forceinline__ uint32_t fp8_to_half2(uint32_t codes) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(codes)));
   return h;
 }
+// Four codes -> the halves of bits 0..15 and of bits 16..31.
+__device__ __forceinline__ void fp8x4_to_half2(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\t"
+      "mov.b32 {l, h}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, l;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %1, h;\n\t}\n"
+      : "=r"(lo), "=r"(hi) : "r"(codes));
+}
 __device__ __forceinline__ float2 fp8_to_float2(uint32_t codes) {
   const uint32_t h = fp8_to_half2(codes & 0xFFFFu);
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
