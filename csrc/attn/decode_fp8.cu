@@ -18,13 +18,15 @@
 //   rescaled rarely.
 // What is behind a sequence's last token never counts: its scores, weights and value bytes are replaced, whatever they are.
 //
-// The split.  The tiles of 64 tokens of all items, in order, are dealt out to four teams per SM, of two consumer warps and a loading one with a
+// The split, many items.  The tiles of 64 tokens of all items, in order, are dealt out to four teams per SM, of two consumer warps and a loading one with a
 // ring each: an item counts as its tiles and kF8ItemCost more for its beginning and end, and team i of C takes the i-th of C equal shares,
 // so short and long contexts, few and many sequences fill the GPU alike.  An item inside one team is finished there; the parts of one that
 // is cut are joined by a second kernel.  Lengths are read on the device, so the launch fits a CUDA graph whatever they become.
 // The four teams of an SM are one CTA: as CTAs of their own, launched beside the end of another kernel (PDL), some SMs took only
 // three, and the others ran after all the rest (256 sequences of 100 .. 1500 tokens: 82 us after an idle GPU, 116 in a row).
-// Bound by memory: 258 bytes per key and KV head.
+// The split, few items of moderate length.  A cluster of one to eight CTAs takes an item, each a run of its tiles of 128 tokens, and they join what they
+// have through distributed shared memory: one launch, and none of the chain from kernel to kernel.
+// Bound by memory: 258 bytes per key and KV head; few items by latency (length -> block table -> keys -> scores -> results).
 #include <algorithm>
 
 #include "../include/fp8_cache.cuh"
@@ -290,9 +292,9 @@ struct F8State {
   __device__ __forceinline__ void finish() {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const float inv = l[h] == 0.f ? 0.f : 1.f / l[h], back = exp2f(u[h] - m[h] - kF8Top);
+      const float f = l[h] == 0.f ? 0.f : 1.f / l[h] * exp2f(u[h] - m[h] - kF8Top);        // (no tokens: no maxima either)
 #pragma unroll
-      for (int k = 0; k < 16; ++k) o[k >> 1][2 * (k & 1) + h] *= inv * back;
+      for (int k = 0; k < 16; ++k) o[k >> 1][2 * (k & 1) + h] *= f;
     }
   }
   __device__ __forceinline__ void store(__nv_bfloat16* rows, int heads, int lane) const {
@@ -537,6 +539,106 @@ __global__ void __launch_bounds__(32 * kF8JoinWarps) decode_fp8_join_kernel(cons
       make_uint2(pack_bf16x2(O.x * inv, O.y * inv), pack_bf16x2(O.z * inv, O.w * inv));
 }
 
+// ---------------------------------------------------------------------------------------------------------
+// Few items: a cluster of CTAs each
+// ---------------------------------------------------------------------------------------------------------
+constexpr int kF8CWarps = 4, kF8CStages = 2, kF8CThreads = 32 * (kF8CWarps + 1), kF8CCtasPerSm = 3;
+using F8ClusterRing = F8Ring<kF8CWarps, kF8CStages>;
+constexpr int f8_cluster_smem(int G) {
+  return 1024 + F8ClusterRing::kBytes + (kF8CWarps - 1) * F8State::kJoinFloats * 4 + G * (kFp8D + 2) * 4 + 2 * kF8CStages * 8;
+}
+
+// Grid (CTAs of an item, items): CTA r of C takes tiles [n r / C, n (r + 1) / C) of its item's n, and its share of the results is what all
+// of them left in their shared memory, joined.
+__global__ void __launch_bounds__(kF8CThreads, kF8CCtasPerSm)
+decode_fp8_cluster_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Fp8Decode a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cap = a.table_width * a.block_size;
+  F8ClusterRing ring;
+  ring.codes = smem;
+  ring.scales = smem + kF8CStages * 2 * F8ClusterRing::kHalf;
+  float* s_join = reinterpret_cast<float*>(smem + F8ClusterRing::kBytes);
+  float* s_o = s_join + (kF8CWarps - 1) * F8State::kJoinFloats;          // [G][128]
+  float* s_ml = s_o + a.G * kFp8D;                                       // [G][2]
+  ring.full = reinterpret_cast<uint64_t*>(s_ml + 2 * a.G);
+  ring.empty = ring.full + kF8CStages;
+  pdl_launch_dependents();
+  if (threadIdx.x == 0) {
+    prefetch_tensormap(&tm_k);
+    prefetch_tensormap(&tm_v);
+    ring.init();
+    fence_mbar_init();
+  }
+  __syncthreads();
+  pdl_wait();
+
+  const int items = a.nkv * a.slices, seq = blockIdx.y / items, item = blockIdx.y - seq * items, rank = blockIdx.x, C = gridDim.x;
+  const int kvh = item / a.slices, slice = item - kvh * a.slices, head0 = kvh * a.group + slice * a.G, heads = min(a.G, a.group - slice * a.G);
+  __nv_bfloat16* out = a.out + (static_cast<size_t>(seq) * a.nq + head0) * kFp8D;
+  int len = a.lens[seq];
+  if (len > cap) {                                       // a corrupted length: clamped and reported
+    if (threadIdx.x == 0) set_status(a.status, kStatusBadIndex);
+    len = cap;
+  }
+  len = max(len, 0);
+  const int n = (len + F8ClusterRing::kTile - 1) / F8ClusterRing::kTile, j = n * rank / C, count = n * (rank + 1) / C - j;
+  if (warp == kF8CWarps) {
+    if (lane == 0) ring.load(a, &tm_k, &tm_v, seq, kvh, len, j, count);
+    __syncwarp();
+  } else {
+    F8State st;
+    st.begin(a.q + (static_cast<size_t>(seq) * a.nq + head0) * kFp8D, heads, a.scale_log2, lane);
+    bool ok = true;
+    for (int i = 0; i < count; ++i, ring.next()) {
+      const int valid = len - (j + i) * F8ClusterRing::kTile - 32 * warp;
+      ok = ok && mbar_wait(&ring.full[ring.s], ring.phase, a.status);
+      if (valid > 0) {
+        const uint8_t* K = ring.codes + ring.s * 2 * F8ClusterRing::kHalf + 32 * warp * kFp8D;
+        const uint8_t* sc = ring.scales + ring.s * 2 * F8ClusterRing::kTile + 32 * warp;
+        st.take(K, K + F8ClusterRing::kHalf, sc, sc + F8ClusterRing::kTile, valid, lane);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ring.empty[ring.s]);
+    }
+    st.sum_up();
+    if (warp > 0) st.publish(s_join + (warp - 1) * F8State::kJoinFloats, lane);
+    named_barrier_sync(1, 32 * kF8CWarps);
+    if (warp == 0) {
+#pragma unroll
+      for (int w = 1; w < kF8CWarps; ++w) st.join(s_join + (w - 1) * F8State::kJoinFloats, lane);
+      st.finish();
+      if (C == 1) st.store(out, heads, lane);
+      else st.store_part(s_o, s_ml, heads, lane);
+    }
+  }
+  if (C == 1) return;
+  __syncwarp();
+  cluster_sync();
+  const int pieces = heads * (kFp8D / 4);                // four dims of a head each
+  for (int i = pieces * rank / C + threadIdx.x; i < pieces * (rank + 1) / C; i += kF8CThreads) {
+    const int head = i / (kFp8D / 4);
+    float M = -INFINITY, L = 0.f;
+    float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+    const uint32_t ml_at = smem_u32(s_ml + 2 * head), o_at = smem_u32(s_o + 4 * i);
+    for (int c = 0; c < C; ++c) M = fmaxf(M, ld_dsmem_f2(dsmem_addr(ml_at, c)).x);
+    for (int c = 0; c < C; ++c) {
+      const float2 ml = ld_dsmem_f2(dsmem_addr(ml_at, c));
+      const float4 v = ld_dsmem_f4(dsmem_addr(o_at, c));
+      const float f = (ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - M)) * ml.y;
+      L += f;
+      O.x = fmaf(f, v.x, O.x);
+      O.y = fmaf(f, v.y, O.y);
+      O.z = fmaf(f, v.z, O.z);
+      O.w = fmaf(f, v.w, O.w);
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    *reinterpret_cast<uint2*>(out + 4 * i) = make_uint2(pack_bf16x2(O.x * inv, O.y * inv), pack_bf16x2(O.z * inv, O.w * inv));
+  }
+  __syncwarp();
+  cluster_sync();                                        // nobody's shared memory goes before it has been read
+}
+
 extern "C" int forge_make_tmap_2d(CUtensorMap* tm, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows, int elem_bytes);
 
 // Grid of a launch of up to 512 sequences; G: query heads of an item.
@@ -555,37 +657,62 @@ static F8Grid f8_grid(int B, int nq, int nkv, int block_size, int table_width) {
   return z;
 }
 
-extern "C" long long forge_decode_fp8_scratch_floats(int B, int nq, int nkv, int block_size, int table_width) {
+// CTAs of an item's cluster, 0: equal shares over the GPU.  mode 1: equal shares, 2: clusters, 0: by size.
+static int f8_cluster(long long items, int table_width, int block_size, int mode) {
+  if (mode == 1 || items > 65535) return 0;
+  const long long slots = static_cast<long long>(kF8CCtasPerSm) * device_sm_count();
+  const long long tiles = (static_cast<long long>(table_width) * block_size + F8ClusterRing::kTile - 1) / F8ClusterRing::kTile;
+  int c = 8;
+  while (c > 1 && (items * c > slots || c > tiles)) c /= 2;
+  return mode == 2 || (items * c <= slots && tiles <= 8 * c) ? c : 0;
+}
+
+// 0: none needed.
+extern "C" long long forge_decode_fp8_scratch_floats(int B, int nq, int nkv, int block_size, int table_width, int mode) {
   const F8Grid z = f8_grid(B, nq, nkv, block_size, table_width);
+  if (f8_cluster(static_cast<long long>(B) * nkv * z.slices, table_width, block_size, mode)) return 0;
   return 2ll * z.teams * z.G * (kFp8D + 2) + 4ll * z.teams;
 }
 
 // q [B, nq, 128], out [B, nq * 128] bf16; a length of zero or less gives a row of zeros.  scratch: forge_decode_fp8_scratch_floats, 16-byte aligned.
 extern "C" int forge_decode_fp8(const void* q, const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales,
                                 const int* block_tables, const int* lens, void* out, float* scratch, int B, int nq, int nkv, int block_size,
-                                int table_width, int num_blocks, float scale, unsigned* status, cudaStream_t stream) {
+                                int table_width, int num_blocks, float scale, int mode, unsigned* status, cudaStream_t stream) {
   if (B <= 0) return 0;
   if (nkv < 1 || nq % nkv != 0 || block_size < 16 || (block_size & (block_size - 1))) return -1;
   const F8Grid z = f8_grid(B, nq, nkv, block_size, table_width);
-  const long long tiles = (static_cast<long long>(table_width) * block_size + F8FlatRing::kTile - 1) / F8FlatRing::kTile;
-  if (std::min(B, kF8Seqs) * (tiles + kF8ItemCost) * nkv * z.slices > INT32_MAX) return -1;
+  Fp8Decode a;
+  a.k_scales = static_cast<const uint8_t*>(k_scales); a.v_scales = static_cast<const uint8_t*>(v_scales);
+  a.nq = nq; a.nkv = nkv; a.group = nq / nkv; a.G = z.G; a.slices = z.slices;
+  a.block_size = block_size; a.table_width = table_width; a.num_blocks = num_blocks;
+  a.scale_log2 = scale * 1.4426950408889634f; a.status = status;
   CUtensorMap tm_k, tm_v;
   const uint64_t rows = static_cast<uint64_t>(num_blocks) * nkv * block_size;
-  const uint32_t box = static_cast<uint32_t>(std::min(block_size, F8FlatRing::kTile));
-  if (forge_make_tmap_2d(&tm_k, k_codes, rows, kFp8D, kFp8D, box, 1) != 0 || forge_make_tmap_2d(&tm_v, v_codes, rows, kFp8D, kFp8D, box, 1) != 0) return -2;
+  const auto maps = [&](int tile) {
+    const uint32_t box = static_cast<uint32_t>(std::min(block_size, tile));
+    return forge_make_tmap_2d(&tm_k, k_codes, rows, kFp8D, kFp8D, box, 1) == 0 && forge_make_tmap_2d(&tm_v, v_codes, rows, kFp8D, kFp8D, box, 1) == 0;
+  };
+  const long long items = static_cast<long long>(B) * nkv * z.slices;
+  if (const int C = f8_cluster(items, table_width, block_size, mode)) {
+    a.q = static_cast<const __nv_bfloat16*>(q); a.block_tables = block_tables; a.lens = lens; a.out = static_cast<__nv_bfloat16*>(out);
+    a.part_o = a.part_ml = nullptr; a.cuts = nullptr; a.B = B;
+    if (!maps(F8ClusterRing::kTile)) return -2;
+    FORGE_ENSURE_DYN_SMEM(decode_fp8_cluster_kernel, f8_cluster_smem(kF8Heads));
+    return launch_kernel_cluster_x(decode_fp8_cluster_kernel, dim3(C, static_cast<unsigned>(items)), dim3(kF8CThreads), f8_cluster_smem(z.G), stream, C,
+                                   tm_k, tm_v, a) == cudaSuccess ? 0 : -5;
+  }
+  const long long tiles = (static_cast<long long>(table_width) * block_size + F8FlatRing::kTile - 1) / F8FlatRing::kTile;
+  if (std::min(B, kF8Seqs) * (tiles + kF8ItemCost) * nkv * z.slices > INT32_MAX) return -1;
+  if (!maps(F8FlatRing::kTile)) return -2;
   FORGE_ENSURE_DYN_SMEM(decode_fp8_kernel, kF8FlatSmem);
+  a.cuts = reinterpret_cast<int4*>(scratch);
+  a.part_o = scratch + 4ll * z.teams;
+  a.part_ml = a.part_o + 2ll * z.teams * z.G * kFp8D;
   for (int b0 = 0; b0 < B; b0 += kF8Seqs) {
-    Fp8Decode a;
     a.q = static_cast<const __nv_bfloat16*>(q) + static_cast<size_t>(b0) * nq * kFp8D;
-    a.k_scales = static_cast<const uint8_t*>(k_scales); a.v_scales = static_cast<const uint8_t*>(v_scales);
     a.block_tables = block_tables + static_cast<size_t>(b0) * table_width; a.lens = lens + b0;
     a.out = static_cast<__nv_bfloat16*>(out) + static_cast<size_t>(b0) * nq * kFp8D;
-    a.cuts = reinterpret_cast<int4*>(scratch);
-    a.part_o = scratch + 4ll * z.teams;
-    a.part_ml = a.part_o + 2ll * z.teams * z.G * kFp8D;
-    a.B = std::min(B - b0, kF8Seqs); a.nq = nq; a.nkv = nkv; a.group = nq / nkv; a.G = z.G; a.slices = z.slices;
-    a.block_size = block_size; a.table_width = table_width; a.num_blocks = num_blocks;
-    a.scale_log2 = scale * 1.4426950408889634f; a.status = status;
+    a.B = std::min(B - b0, kF8Seqs);
     if (launch_kernel(decode_fp8_kernel, dim3(z.ctas), dim3(kF8Threads), kF8FlatSmem, stream, 0, tm_k, tm_v, a) != cudaSuccess) return -5;
     if (launch_kernel(decode_fp8_join_kernel, dim3(z.teams), dim3(32 * kF8JoinWarps), 0, stream, 0, a) != cudaSuccess) return -5;
   }

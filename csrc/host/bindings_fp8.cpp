@@ -18,8 +18,8 @@ int forge_fp8_expand(const void* k_codes, const void* k_scales, const void* v_co
                      int* tables, int capacity, unsigned* status, cudaStream_t stream);
 int forge_decode_fp8(const void* q, const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales,
                      const int* block_tables, const int* lens, void* out, float* scratch, int B, int nq, int nkv, int block_size, int table_width,
-                     int num_blocks, float scale, unsigned* status, cudaStream_t stream);
-long long forge_decode_fp8_scratch_floats(int B, int nq, int nkv, int block_size, int table_width);
+                     int num_blocks, float scale, int mode, unsigned* status, cudaStream_t stream);
+long long forge_decode_fp8_scratch_floats(int B, int nq, int nkv, int block_size, int table_width, int mode);
 int forge_rms_norm_fp8(const void* x, void* residual, const void* w, void* codes, float* scales, int scale_ld, int rows, int H, float eps,
                        cudaStream_t stream);
 }
@@ -113,9 +113,9 @@ std::tuple<Tensor, Tensor, Tensor> fp8_expand(const Tensor& k_codes, const Tenso
   return {k_out, v_out, tables};
 }
 
-// Returns [sequences, nq * 128].
+// Returns [sequences, nq * 128].  mode: 0 by size, 1 equal shares over the GPU, 2 a cluster of CTAs per sequence and KV head.
 Tensor decode_fp8(const Tensor& q, const Tensor& k_codes, const Tensor& k_scales, const Tensor& v_codes, const Tensor& v_scales,
-                  const Tensor& block_tables, const Tensor& lens, double scale, const Tensor& status) {
+                  const Tensor& block_tables, const Tensor& lens, double scale, const Tensor& status, int64_t mode) {
   const Half k = cache_half(k_codes, k_scales, q, "decode_fp8"), v = cache_half(v_codes, v_scales, q, "decode_fp8");
   TORCH_CHECK(k_codes.sizes() == v_codes.sizes(), "decode_fp8: keys and values of one shape expected");
   TORCH_CHECK(q.dim() == 3 && q.size(2) == 128 && block_tables.dim() == 2, "decode_fp8: q must be [sequences, heads, 128], tables [sequences, width]");
@@ -130,9 +130,11 @@ Tensor decode_fp8(const Tensor& q, const Tensor& k_codes, const Tensor& k_scales
   const int* ln = ints(lens, B, "decode_fp8: lengths");
   const c10::cuda::CUDAGuard guard(q.device());
   Tensor out = at::empty({B, nq * 128}, q.options());
-  const Tensor scratch = at::empty({forge_decode_fp8_scratch_floats(i32(B), i32(nq), i32(k.nkv), i32(k.block), i32(W))}, q.options().dtype(at::kFloat));
-  check_rc(forge_decode_fp8(qp, k.codes, k.scales, v.codes, v.scales, bt, ln, out.data_ptr(), scratch.data_ptr<float>(), i32(B), i32(nq), i32(k.nkv),
-                            i32(k.block), i32(W), i32(k.blocks), static_cast<float>(scale), status_word(status), stream_of(q)),
+  const int64_t floats = forge_decode_fp8_scratch_floats(i32(B), i32(nq), i32(k.nkv), i32(k.block), i32(W), i32(mode));
+  Tensor scratch;
+  if (floats > 0) scratch = at::empty({floats}, q.options().dtype(at::kFloat));
+  check_rc(forge_decode_fp8(qp, k.codes, k.scales, v.codes, v.scales, bt, ln, out.data_ptr(), floats > 0 ? scratch.data_ptr<float>() : nullptr, i32(B), i32(nq),
+                            i32(k.nkv), i32(k.block), i32(W), i32(k.blocks), static_cast<float>(scale), i32(mode), status_word(status), stream_of(q)),
            "forge_decode_fp8");
   return out;
 }

@@ -220,7 +220,9 @@ def test_every_code_and_scale_reads_back_exactly(ops):
     ([700, 2011, 129, 128], 32, 8, 256), ([300, 1000, 70, 2], 40, 8, 128), ([129, 640, 33], 64, 8, 256), ([50, 400], 6, 2, 64), ([255, 256, 257], 7, 1, 64),
     ([300, 65, 2], 10, 1, 64), ([700, 129], 24, 2, 256), ([64, 513], 32, 2, 16), ([100] * 70, 5, 1, 32), ([9001, 3], 12, 4, 256), ([0, 0, 0], 4, 2, 64),
 ])
-def test_decode(ops, lens, nq, nkv, bs):
+@pytest.mark.parametrize("mode", ["flat", "chunked", "auto"])
+def test_decode(ops, lens, nq, nkv, bs, mode, monkeypatch):
+    monkeypatch.setattr(ops, "decode_attention_mode", mode)
     q, kc, vc, step = _paged(lens, nq, nkv, bs)
     got = ops.attention(q, kc, vc, step, SCALE)
     ops.check_status()
@@ -238,15 +240,19 @@ def test_decode_of_many_sequences(ops, batch, lo, hi, nq, nkv):
 
 
 @pytest.mark.parametrize("scale", [0.0, -0.05, 1.0])
-def test_decode_with_other_scales(ops, scale):
+@pytest.mark.parametrize("mode", ["flat", "chunked"])
+def test_decode_with_other_scales(ops, scale, mode, monkeypatch):
+    monkeypatch.setattr(ops, "decode_attention_mode", mode)
     lens = [300, 1, 1000]
     q, kc, vc, step = _paged(lens, 8, 2, 64)
     _check_decode(ops.attention(q, kc, vc, step, scale), q, kc, vc, step, lens, scale)
 
 
 @pytest.mark.parametrize("spread,q_scale", [(12.0, 1e-3), (0.0, 300.0), (3.0, 1e-30), (0.5, 1e30)])
-def test_decode_with_far_apart_scales(ops, spread, q_scale):
+@pytest.mark.parametrize("mode", ["flat", "chunked"])
+def test_decode_with_far_apart_scales(ops, spread, q_scale, mode, monkeypatch):
     """Values and keys whose heads differ by many powers of two, and queries of extreme sizes."""
+    monkeypatch.setattr(ops, "decode_attention_mode", mode)
     lens = [500, 2, 77]
     q, kc, vc, step = _paged(lens, 8, 2, 64, spread=spread, q_scale=q_scale)
     scale = SCALE / q_scale
@@ -256,8 +262,10 @@ def test_decode_with_far_apart_scales(ops, spread, q_scale):
     _check_decode(ops.attention(q, kc, vc, step, scale), q, kc, vc, step, lens, scale)
 
 
-def test_decode_with_rising_and_falling_scores(ops):
+@pytest.mark.parametrize("mode", ["flat", "chunked"])
+def test_decode_with_rising_and_falling_scores(ops, mode, monkeypatch):
     """Maxima that rise at every token, by little and by much, and a first token that outweighs all others."""
+    monkeypatch.setattr(ops, "decode_attention_mode", mode)
     for seed, slope in ((0, 0.004), (1, 0.3), (2, -0.3), (3, 3.0)):
         lens = [700, 130, 33]
         q, kc, vc, step = _paged(lens, 8, 2, 64, seed=seed)
@@ -274,7 +282,9 @@ def test_decode_with_rising_and_falling_scores(ops):
         _check_decode(ops.attention(q, kc, vc, step, SCALE), q, kc, vc, step, lens)
 
 
-def test_decode_keeps_nan_where_it_belongs(ops):
+@pytest.mark.parametrize("mode", ["flat", "chunked"])
+def test_decode_keeps_nan_where_it_belongs(ops, mode, monkeypatch):
+    monkeypatch.setattr(ops, "decode_attention_mode", mode)
     lens = [300, 70, 200, 40]
     q, kc, vc, step = _paged(lens, 8, 2, 64)
     want = ops.attention(q, kc, vc, step, SCALE).view(4, 8, 128)
@@ -294,7 +304,9 @@ def test_decode_keeps_nan_where_it_belongs(ops):
     assert torch.equal(got[~bad], want[~bad])
 
 
-def test_decode_reports_lengths_and_blocks_that_do_not_exist(ops):
+@pytest.mark.parametrize("mode", ["flat", "chunked"])
+def test_decode_reports_lengths_and_blocks_that_do_not_exist(ops, mode, monkeypatch):
+    monkeypatch.setattr(ops, "decode_attention_mode", mode)
     lens = [300, 100, 520]
     q, kc, vc, step = _paged(lens, 8, 2, 64)
     step.context_lens[1] = 64 * step.table_width + 1
@@ -312,7 +324,9 @@ def test_decode_reports_lengths_and_blocks_that_do_not_exist(ops):
         _check_decode(other[[0, 2]], q[[0, 2]], kc, vc, Step(block_tables=step.block_tables[[0, 2]]), [300, 520])
 
 
-def test_decode_negative_lengths_and_padding_rows_are_zero(ops):
+@pytest.mark.parametrize("mode", ["flat", "chunked"])
+def test_decode_negative_lengths_and_padding_rows_are_zero(ops, mode, monkeypatch):
+    monkeypatch.setattr(ops, "decode_attention_mode", mode)
     lens = [65, 0, 3]
     q, kc, vc, step = _paged(lens, 16, 8, 16)
     step.context_lens[1] = -7
@@ -420,7 +434,9 @@ def test_refusals(ops):
 
 
 # ----------------------------------------------------------------------------- streams, graphs, order
-def test_decode_gives_the_same_bits_again_and_on_another_stream(ops):
+@pytest.mark.parametrize("mode", ["flat", "chunked"])
+def test_decode_gives_the_same_bits_again_and_on_another_stream(ops, mode, monkeypatch):
+    monkeypatch.setattr(ops, "decode_attention_mode", mode)
     q, kc, vc, step = _paged([3001, 64, 700], 32, 8, 256)
     want = ops.attention(q, kc, vc, step, SCALE)
     side = torch.cuda.Stream()
@@ -432,8 +448,10 @@ def test_decode_gives_the_same_bits_again_and_on_another_stream(ops):
     assert all(torch.equal(a, want) for a in (*again, here))
 
 
-def test_captured_steps_follow_their_inputs(ops):
+@pytest.mark.parametrize("mode", ["flat", "chunked"])
+def test_captured_steps_follow_their_inputs(ops, mode, monkeypatch):
     """Two graphs of different batches, replayed in turn and over other lengths, beside an eager call."""
+    monkeypatch.setattr(ops, "decode_attention_mode", mode)
     cases = []
     for lens, nq, nkv, seed in (([700, 65, 1], 32, 8, 0), ([300] * 5, 16, 8, 1)):
         q, kc, vc, step = _paged(lens, nq, nkv, 64, seed=seed)

@@ -8,6 +8,8 @@ import torch
 
 from .quant import Fp8KVCache, Fp8Rows
 
+_DECODE_MODES = {"auto": 0, "flat": 1, "chunked": 2}
+
 
 class Fp8Ops:
     """Mixed into ``CudaOps`` (uses its ``C``, ``status``, ``device`` and ``num_sms``)."""
@@ -31,7 +33,9 @@ class Fp8Ops:
         return self.C.fp8_expand(*self._halves(k_cache, v_cache), block_tables, context_lens, num_pages, self.status)
 
     def decode_attention_fp8(self, q, k_cache, v_cache, batch, scale):
-        return self.C.decode_fp8(q, *self._halves(k_cache, v_cache), batch.block_tables, batch.context_lens, scale, self.status)
+        """``decode_attention_mode``: "flat" equal shares over the GPU, "chunked" a cluster of CTAs per sequence and KV head, "auto" by size."""
+        return self.C.decode_fp8(q, *self._halves(k_cache, v_cache), batch.block_tables, batch.context_lens, scale, self.status,
+                                 _DECODE_MODES[self.decode_attention_mode])
 
     def prefill_attention_fp8(self, q, k_cache, v_cache, batch, scale):
         """Prompts: the sequences' pages are read back and attended to by the bf16 kernels, as many sequences at a time as have
