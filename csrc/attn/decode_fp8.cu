@@ -332,6 +332,7 @@ struct F8State {
 constexpr int kF8Warps = 2, kF8Stages = 3, kF8Teams = 4;
 constexpr int kF8TeamWarps = kF8Warps + 1, kF8Threads = 32 * kF8Teams * kF8TeamWarps;
 constexpr int kF8ItemCost = 2;                         // tiles
+constexpr int kF8Share = 4;                            // no team gets less than this
 using F8FlatRing = F8Ring<kF8Warps, kF8Stages>;
 
 constexpr int kF8JoinArea = (kF8Warps - 1) * F8State::kJoinFloats;
@@ -419,7 +420,7 @@ decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     __syncthreads();
   }
   const int items = a.nkv * a.slices, units = s_before[a.B] * items;
-  const int me = team * gridDim.x + blockIdx.x, workers = min(static_cast<int>(kF8Teams * gridDim.x), units);
+  const int me = team * gridDim.x + blockIdx.x, workers = min(static_cast<int>(kF8Teams * gridDim.x), (units + kF8Share - 1) / kF8Share);
   for (int b = blockIdx.x; b < a.B; b += gridDim.x)    // rows without tokens: zeros
     if (s_before[b + 1] == s_before[b])
       for (int i = threadIdx.x; i < a.nq * kFp8D / 8; i += kF8Threads)
@@ -491,7 +492,7 @@ decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   }
 }
 
-// Joins the parts of an item that was cut: one or more warps per head take its parts in turn.
+// Joins the parts of an item that was cut.  A CTA for a cut and a head, its warps take the parts in turn.
 constexpr int kF8JoinWarps = 8;
 
 __global__ void __launch_bounds__(32 * kF8JoinWarps) decode_fp8_join_kernel(const Fp8Decode a) {
@@ -499,43 +500,40 @@ __global__ void __launch_bounds__(32 * kF8JoinWarps) decode_fp8_join_kernel(cons
   __shared__ float s_l[kF8JoinWarps];
   pdl_launch_dependents();
   pdl_wait();
-  const int me = blockIdx.x;
+  const int me = blockIdx.x, head = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int4 cut = a.cuts[me];
-  const int parts = cut.x;
-  if (parts == 0) return;
-  const int kvh = cut.z / a.slices, slice = cut.z - kvh * a.slices, heads = min(a.G, a.group - slice * a.G), head0 = kvh * a.group + slice * a.G;
-  const int per_head = a.G <= 1 ? 8 : a.G <= 2 ? 4 : a.G <= 4 ? 2 : 1;   // warps
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, head = warp / per_head, sub = warp % per_head;
-  auto slot = [&](int i) { return static_cast<size_t>(i == 0 ? 2 * (me - 1) + 1 : 2 * (me + i - 1)) * a.G + head; };
+  const int parts = cut.x, kvh = cut.z / a.slices, slice = cut.z - kvh * a.slices;
+  if (parts == 0 || head >= min(a.G, a.group - slice * a.G)) return;
+  const auto slot = [&](int i) { return static_cast<size_t>(i == 0 ? 2 * (me - 1) + 1 : 2 * (me + i - 1)) * a.G + head; };
   float M = -INFINITY, L = 0.f;
   float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (head < heads) {
-    for (int i = lane; i < parts; i += 32) M = fmaxf(M, a.part_ml[2 * slot(i)]);
+  for (int i = lane; i < parts; i += 32) M = fmaxf(M, a.part_ml[2 * slot(i)]);
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+  for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
 #pragma unroll 4
-    for (int i = sub; i < parts; i += per_head) {
-      const size_t p = slot(i);
-      const float mi = a.part_ml[2 * p], f = (mi == -INFINITY ? 0.f : exp2f(mi - M)) * a.part_ml[2 * p + 1];
-      const float4 v = *reinterpret_cast<const float4*>(a.part_o + p * kFp8D + 4 * lane);
-      L += f;
-      O.x = fmaf(f, v.x, O.x);
-      O.y = fmaf(f, v.y, O.y);
-      O.z = fmaf(f, v.z, O.z);
-      O.w = fmaf(f, v.w, O.w);
-    }
+  for (int i = warp; i < parts; i += kF8JoinWarps) {
+    const size_t p = slot(i);
+    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * p);
+    const float4 v = *reinterpret_cast<const float4*>(a.part_o + p * kFp8D + 4 * lane);
+    const float f = (ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - M)) * ml.y;
+    L += f;
+    O.x = fmaf(f, v.x, O.x);
+    O.y = fmaf(f, v.y, O.y);
+    O.z = fmaf(f, v.z, O.z);
+    O.w = fmaf(f, v.w, O.w);
   }
   s_o[warp][lane] = O;
   if (lane == 0) s_l[warp] = L;
   __syncthreads();
-  if (head >= heads || sub != 0) return;
-  for (int i = 1; i < per_head; ++i) {
-    const float4 v = s_o[warp + i][lane];
+  if (warp != 0) return;
+  for (int i = 1; i < min(kF8JoinWarps, parts); ++i) {
+    const float4 v = s_o[i][lane];
     O.x += v.x; O.y += v.y; O.z += v.z; O.w += v.w;
-    L += s_l[warp + i];
+    L += s_l[i];
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;
-  *reinterpret_cast<uint2*>(a.out + (static_cast<size_t>(cut.y) * a.nq + head0 + head) * kFp8D + 4 * lane) =
+  const int h = kvh * a.group + slice * a.G + head;
+  *reinterpret_cast<uint2*>(a.out + (static_cast<size_t>(cut.y) * a.nq + h) * kFp8D + 4 * lane) =
       make_uint2(pack_bf16x2(O.x * inv, O.y * inv), pack_bf16x2(O.z * inv, O.w * inv));
 }
 
@@ -657,14 +655,19 @@ static F8Grid f8_grid(int B, int nq, int nkv, int block_size, int table_width) {
   return z;
 }
 
-// CTAs of an item's cluster, 0: equal shares over the GPU.  mode 1: equal shares, 2: clusters, 0: by size.
+// CTAs of an item's cluster, 0: equal shares over the GPU.  mode 1: equal shares, 2: clusters, 0: by size, the longest context being as long as the
+// block table is wide.  Measured, equal shares / clusters, us: 32 / 8 heads, 1 x 700 10.0 / 6.3, 1 x 4096 11.3 / 8.8, 1 x 16000 15.0 / 21.4, 4 x 4000
+// 13.4 / 10.7, 8 x 200 .. 2000 (64 items, clusters of 4) 12.6 / 9.8, 13 x 200 .. 2000 (104) 13.2 / 15.7, 24 x 200 .. 2000 17.0 / 20.3; 8 / 1 heads, 32 x
+// 200 .. 2000 (clusters of 8) 14.2 / 7.8; contexts of four tiles, 64 x 100 .. 500 17.2 / 15.4, 100 x 100 .. 300 18.2 / 17.6.  Clusters of 8 find no
+// place beside each other long before all SMs are taken, hence the bound of 256 CTAs (with two CTAs per SM 32 clusters took 16.1 for 7.8); clusters
+// of 16 were no faster where eight fit (1 x 3001: 7.9), and 11.5 for 6.7 where they did not.
 static int f8_cluster(long long items, int table_width, int block_size, int mode) {
+  constexpr int kCtas = 256, kTilesOfOne = 4, kTiles = 8;
   if (mode == 1 || items > 65535) return 0;
-  const long long slots = static_cast<long long>(kF8CCtasPerSm) * device_sm_count();
   const long long tiles = (static_cast<long long>(table_width) * block_size + F8ClusterRing::kTile - 1) / F8ClusterRing::kTile;
   int c = 8;
-  while (c > 1 && (items * c > slots || c > tiles)) c /= 2;
-  return mode == 2 || (items * c <= slots && tiles <= 8 * c) ? c : 0;
+  while (c > 1 && (items * c > kCtas || c > tiles)) c /= 2;
+  return mode == 2 || tiles <= kTilesOfOne || (c >= 4 && tiles <= kTiles * c) ? c : 0;
 }
 
 // 0: none needed.
@@ -714,7 +717,7 @@ extern "C" int forge_decode_fp8(const void* q, const void* k_codes, const void* 
     a.out = static_cast<__nv_bfloat16*>(out) + static_cast<size_t>(b0) * nq * kFp8D;
     a.B = std::min(B - b0, kF8Seqs);
     if (launch_kernel(decode_fp8_kernel, dim3(z.ctas), dim3(kF8Threads), kF8FlatSmem, stream, 0, tm_k, tm_v, a) != cudaSuccess) return -5;
-    if (launch_kernel(decode_fp8_join_kernel, dim3(z.teams), dim3(32 * kF8JoinWarps), 0, stream, 0, a) != cudaSuccess) return -5;
+    if (launch_kernel(decode_fp8_join_kernel, dim3(z.teams, z.G), dim3(32 * kF8JoinWarps), 0, stream, 0, a) != cudaSuccess) return -5;
   }
   return 0;
 }
