@@ -7,6 +7,8 @@
 //            values whether its prefix was cached or written a moment ago.
 //
 // No counterpart in the reference, whose cache has the model's type.
+#include <algorithm>
+
 #include "../include/fp8_cache.cuh"
 #include "../include/launch.cuh"
 #include "../include/ptx.cuh"
@@ -42,23 +44,31 @@ struct Fp8Store {
   uint8_t *k_codes, *k_scales, *v_codes, *v_scales;
   int T, nq, nkv, block_size;
   long long num_slots;
-  int heads_per_warp;
   unsigned* status;
 };
 
-// Eight lanes per head, lane j of them has entries 8j.. and 64 + 8j.., the pairs that the rotation mixes; a warp works on four heads
-// of a token at a time, `heads_per_warp` in all, so that position, slot and angles are fetched once.  Bound by memory: qkv read once,
-// q and the codes written once.
-template <bool kVec>
+// Eight lanes per head, lane j of them has entries 8j.. and 64 + 8j.., the pairs that the rotation mixes; a warp works on kSets sets of
+// four heads of a token, all of whose loads are under way at once, and fetches position, slot and angles once.  Bound by memory: qkv
+// read once, q and the codes written once.
+template <bool kVec, int kSets>
 __global__ void __launch_bounds__(128) fp8_store_kernel(const Fp8Store a) {
   pdl_launch_dependents();
   pdl_wait();
-  const int heads = a.nq + 2 * a.nkv, groups = (heads + a.heads_per_warp - 1) / a.heads_per_warp;
+  const int heads = a.nq + 2 * a.nkv, groups = (heads + 4 * kSets - 1) / (4 * kSets);
   const long long wid = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
   if (wid >= static_cast<long long>(a.T) * groups) return;
   const int lane = threadIdx.x & 31, j = lane & 7, sub = lane >> 3;
-  const int t = static_cast<int>(wid / groups);
-  const int h_begin = static_cast<int>(wid % groups) * a.heads_per_warp, h_end = min(h_begin + a.heads_per_warp, heads);
+  const int t = static_cast<int>(wid / groups), h0 = static_cast<int>(wid - static_cast<long long>(t) * groups) * 4 * kSets + sub;
+  float lo[kSets][8], hi[kSets][8];
+#pragma unroll
+  for (int k = 0; k < kSets; ++k) {
+    const __nv_bfloat16* src = a.qkv + static_cast<size_t>(t) * a.ld + static_cast<size_t>(min(h0 + 4 * k, heads - 1)) * kFp8D + 8 * j;
+    load8<kVec>(src, lo[k]);
+    load8<kVec>(src + 64, hi[k]);
+  }
+  const long long slot = a.slots[t];
+  const bool slot_ok = slot >= 0 && slot < a.num_slots;
+  if (slot >= a.num_slots && lane == 0) set_status(a.status, kStatusBadIndex);
   float c[8], s[8];
   if (a.rope != nullptr) {
     const float* cs = a.rope + static_cast<size_t>(min(max(a.positions[t], 0), a.rope_rows - 1)) * kFp8D;
@@ -68,21 +78,15 @@ __global__ void __launch_bounds__(128) fp8_store_kernel(const Fp8Store a) {
       *reinterpret_cast<float4*>(s + i) = *reinterpret_cast<const float4*>(cs + 64 + 8 * j + i);
     }
   }
-  const long long slot = a.slots[t];
-  const bool slot_ok = slot >= 0 && slot < a.num_slots;
-  if (slot >= a.num_slots && lane == 0) set_status(a.status, kStatusBadIndex);
-
-  for (int h0 = h_begin; h0 < h_end; h0 += 4) {
-    const int h = h0 + sub;
-    const bool live = h < h_end, is_q = h < a.nq, is_k = !is_q && h < a.nq + a.nkv;
-    const __nv_bfloat16* src = a.qkv + static_cast<size_t>(t) * a.ld + static_cast<size_t>(live ? h : h_begin) * kFp8D;
-    float lo[8], hi[8];
-    load8<kVec>(src + 8 * j, lo);
-    load8<kVec>(src + 64 + 8 * j, hi);
+#pragma unroll
+  for (int k = 0; k < kSets; ++k) {
+    const int h = h0 + 4 * k;
+    const bool is_q = h < a.nq, is_k = !is_q && h < a.nq + a.nkv;
+    float (&x)[8] = lo[k], (&y)[8] = hi[k];
     const __nv_bfloat16* w = is_q ? a.qw : is_k ? a.kw : nullptr;
     float ss = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss = add_squares(lo[i], hi[i], ss);
+    for (int i = 0; i < 8; ++i) ss = add_squares(x[i], y[i], ss);
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
     if (w != nullptr) {
@@ -92,41 +96,49 @@ __global__ void __launch_bounds__(128) fp8_store_kernel(const Fp8Store a) {
       load8<kVec>(w + 64 + 8 * j, wh);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        lo[i] = lo[i] * inv * wl[i];
-        hi[i] = hi[i] * inv * wh[i];
+        x[i] = x[i] * inv * wl[i];
+        y[i] = y[i] * inv * wh[i];
       }
     }
     if (a.rope != nullptr && (is_q || is_k)) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) rotate_pair(lo[i], hi[i], c[i], s[i]);
+      for (int i = 0; i < 8; ++i) rotate_pair(x[i], y[i], c[i], s[i]);
     }
     uint32_t amax = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) amax = max(amax, max(abs_bits(lo[i]), abs_bits(hi[i])));
+    for (int i = 0; i < 8; ++i) amax = max(amax, max(abs_bits(x[i]), abs_bits(y[i])));
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    if (!live) continue;
+    if (h >= heads) continue;
     if (is_q) {
       __nv_bfloat16* dst = a.q_out + (static_cast<size_t>(t) * a.nq + h) * kFp8D + 8 * j;
-      *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16x2(lo[0], lo[1]), pack_bf16x2(lo[2], lo[3]), pack_bf16x2(lo[4], lo[5]), pack_bf16x2(lo[6], lo[7]));
-      *reinterpret_cast<uint4*>(dst + 64) = make_uint4(pack_bf16x2(hi[0], hi[1]), pack_bf16x2(hi[2], hi[3]), pack_bf16x2(hi[4], hi[5]), pack_bf16x2(hi[6], hi[7]));
+      *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+      *reinterpret_cast<uint4*>(dst + 64) = make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7]));
       continue;
     }
     if (!slot_ok) continue;
     const int kvh = is_k ? h - a.nq : h - a.nq - a.nkv;
-    const size_t row = (static_cast<size_t>(slot / a.block_size) * a.nkv + kvh) * a.block_size + slot % a.block_size;
+    const long long block = slot / a.block_size;
+    const size_t row = (static_cast<size_t>(block) * a.nkv + kvh) * a.block_size + (slot - block * a.block_size);
     const uint32_t b = fp8_scale_byte(amax);
     uint2 code[2] = {make_uint2(kCodesNan, kCodesNan), make_uint2(kCodesNan, kCodesNan)};
     if (b != kScaleNan) {
       const float m = fp8_inverse_scale(b);
-      code[0] = make_uint2(fp8_pack(lo[0] * m, lo[1] * m, lo[2] * m, lo[3] * m), fp8_pack(lo[4] * m, lo[5] * m, lo[6] * m, lo[7] * m));
-      code[1] = make_uint2(fp8_pack(hi[0] * m, hi[1] * m, hi[2] * m, hi[3] * m), fp8_pack(hi[4] * m, hi[5] * m, hi[6] * m, hi[7] * m));
+      code[0] = make_uint2(fp8_pack(x[0] * m, x[1] * m, x[2] * m, x[3] * m), fp8_pack(x[4] * m, x[5] * m, x[6] * m, x[7] * m));
+      code[1] = make_uint2(fp8_pack(y[0] * m, y[1] * m, y[2] * m, y[3] * m), fp8_pack(y[4] * m, y[5] * m, y[6] * m, y[7] * m));
     }
     uint8_t* dst = (is_k ? a.k_codes : a.v_codes) + row * kFp8D + 8 * j;
     *reinterpret_cast<uint2*>(dst) = code[0];
     *reinterpret_cast<uint2*>(dst + 64) = code[1];
     if (j == 0) (is_k ? a.k_scales : a.v_scales)[row] = static_cast<uint8_t>(b);
   }
+}
+
+template <bool kVec, int kSets>
+static int launch_store(const Fp8Store& a, cudaStream_t stream) {
+  const int groups = (a.nq + 2 * a.nkv + 4 * kSets - 1) / (4 * kSets);
+  const dim3 grid(static_cast<unsigned>((static_cast<long long>(a.T) * groups + 3) / 4));
+  return launch_kernel(fp8_store_kernel<kVec, kSets>, grid, dim3(128), 0, stream, 0, a) == cudaSuccess ? 0 : -2;
 }
 
 // qkv [T, (nq + 2 nkv) * 128] with rows ld apart; rope fp32 [rope_rows][128] = cos, sin; slot < 0 is passed over, slot >= num_slots too and
@@ -143,18 +155,17 @@ extern "C" int forge_fp8_store(const void* qkv, long long ld, const void* qw, co
   a.k_codes = static_cast<uint8_t*>(k_codes); a.k_scales = static_cast<uint8_t*>(k_scales);
   a.v_codes = static_cast<uint8_t*>(v_codes); a.v_scales = static_cast<uint8_t*>(v_scales);
   a.T = T; a.nq = nq; a.nkv = nkv; a.block_size = block_size; a.num_slots = num_slots; a.status = status;
-  a.heads_per_warp = T >= 4096 ? 16 : T >= 512 ? 8 : 4;
-  const int groups = (nq + 2 * nkv + a.heads_per_warp - 1) / a.heads_per_warp;
-  const dim3 grid(static_cast<unsigned>((static_cast<long long>(T) * groups + 3) / 4));
   auto aligned = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
   const bool vec = ld % 8 == 0 && aligned(qkv) && aligned(qw) && aligned(kw);
-  return launch_kernel(vec ? fp8_store_kernel<true> : fp8_store_kernel<false>, grid, dim3(128), 0, stream, 0, a) == cudaSuccess ? 0 : -2;
+  if (!vec) return launch_store<false, 1>(a, stream);
+  return T < 512 ? launch_store<true, 1>(a, stream) : launch_store<true, 2>(a, stream);
 }
 
 // ---------------------------------------------------------------------------------------------------------
-// Pages of sequences, in order, as bf16.  A CTA takes `rows` token rows of one page of one head of K or V.
+// Pages of sequences, in order, as bf16.  A CTA takes `rows` token rows of one page of one head of K or V.  Lengths, table entry and, once the
+// latter is there, the codes are asked for one after the other; where the page goes is found out meanwhile.  Bound by memory.
 // ---------------------------------------------------------------------------------------------------------
-constexpr int kExpandThreads = 256;
+constexpr int kExpandThreads = 256, kExpandLoads = 4;
 
 __global__ void __launch_bounds__(kExpandThreads) fp8_expand_kernel(
     const uint8_t* __restrict__ k_codes, const uint8_t* __restrict__ k_scales, const uint8_t* __restrict__ v_codes,
@@ -162,25 +173,46 @@ __global__ void __launch_bounds__(kExpandThreads) fp8_expand_kernel(
     int nkv, int block_size, int rows, __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out, int* __restrict__ tables,
     int capacity, unsigned* status) {
   __shared__ int red[kExpandThreads / 32];
-  pdl_launch_dependents();
-  pdl_wait();
   const int seq = blockIdx.y, page = blockIdx.x;
   const int parts = block_size / rows, z = blockIdx.z;
   const int part = z % parts, kvh = z / parts % nkv, is_v = z / parts / nkv;
   const int cap = table_width * block_size;
-  const bool first_cta = z == 0;
+  const bool scribe = z == 0 && threadIdx.x == 0;       // writes the page's table entry
+  pdl_launch_dependents();
+  pdl_wait();
   int len = lens[seq];
-  if (len > cap) {
-    if (first_cta && page == 0 && threadIdx.x == 0) set_status(status, kStatusBadIndex);
-    len = cap;
-  }
-  const int need = (max(len, 0) + block_size - 1) / block_size;
-  if (page >= need) {
-    if (first_cta && threadIdx.x == 0) tables[static_cast<size_t>(seq) * table_width + page] = -1;
-    return;
-  }
+  int blk = block_tables[static_cast<size_t>(seq) * table_width + page];
   int before = 0;                                       // pages of the sequences before this one
   for (int i = threadIdx.x; i < seq; i += kExpandThreads) before += (min(max(lens[i], 0), cap) + block_size - 1) / block_size;
+  if (len > cap) {
+    if (scribe && page == 0) set_status(status, kStatusBadIndex);
+    len = cap;
+  }
+  int* entry = tables + static_cast<size_t>(seq) * table_width + page;
+  if (page * block_size >= len) {
+    if (scribe) *entry = -1;
+    return;
+  }
+  if (blk < 0 || blk >= num_blocks) {
+    if (scribe) set_status(status, kStatusBadIndex);
+    blk = 0;
+  }
+  const size_t row0 = (static_cast<size_t>(blk) * nkv + kvh) * block_size + part * rows;
+  const int live = min(len - page * block_size - part * rows, rows);
+  const uint8_t* codes = (is_v ? v_codes : k_codes) + row0 * kFp8D;
+  const uint8_t* scales = (is_v ? v_scales : k_scales) + row0;
+  uint4 raw[kExpandLoads];
+  uint32_t scale[kExpandLoads];
+  const auto fetch = [&](int i0) {                      // 16 codes each; zeros behind the last token
+#pragma unroll
+    for (int k = 0; k < kExpandLoads; ++k) {
+      const int i = i0 + k * kExpandThreads;
+      const bool in = i >> 3 < live;
+      raw[k] = in ? *reinterpret_cast<const uint4*>(codes + static_cast<size_t>(i) * 16) : make_uint4(0, 0, 0, 0);
+      scale[k] = in ? scales[i >> 3] : 0u;
+    }
+  };
+  fetch(threadIdx.x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = before;
@@ -190,40 +222,33 @@ __global__ void __launch_bounds__(kExpandThreads) fp8_expand_kernel(
   for (int i = 0; i < kExpandThreads / 32; ++i) before += red[i];
   const int to = before + page;
   if (to >= capacity) {
-    if (first_cta && threadIdx.x == 0) {
+    if (scribe) {
       set_status(status, kStatusBadIndex);
-      tables[static_cast<size_t>(seq) * table_width + page] = -1;
+      *entry = -1;
     }
     return;
   }
-  int blk = block_tables[static_cast<size_t>(seq) * table_width + page];
-  if (blk < 0 || blk >= num_blocks) {
-    if (first_cta && threadIdx.x == 0) set_status(status, kStatusBadIndex);
-    blk = 0;
-  }
-  if (first_cta && threadIdx.x == 0) tables[static_cast<size_t>(seq) * table_width + page] = to;
-  const size_t row0 = (static_cast<size_t>(blk) * nkv + kvh) * block_size + part * rows;
-  const size_t out0 = (static_cast<size_t>(to) * nkv + kvh) * block_size + part * rows;
-  const int live = min(len - page * block_size - part * rows, rows);
-  const uint8_t* codes = (is_v ? v_codes : k_codes) + row0 * kFp8D;
-  const uint8_t* scales = (is_v ? v_scales : k_scales) + row0;
-  __nv_bfloat16* out = (is_v ? v_out : k_out) + out0 * kFp8D;
-  for (int i = threadIdx.x; i < rows * 8; i += kExpandThreads) {                // 16 codes each
-    const int r = i >> 3;
-    uint32_t o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (r < live) {
-      const uint4 raw = *reinterpret_cast<const uint4*>(codes + i * 16);
-      const float m = fp8_scale(scales[r]);
-      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  if (scribe) *entry = to;
+  __nv_bfloat16* out = (is_v ? v_out : k_out) + ((static_cast<size_t>(to) * nkv + kvh) * block_size + part * rows) * kFp8D;
+  for (int i0 = threadIdx.x; i0 < rows * 8; i0 += kExpandLoads * kExpandThreads) {
+    if (i0 != threadIdx.x) fetch(i0);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float2 f = fp8_to_float2(w[e >> 1] >> (16 * (e & 1)));
-        o[e] = pack_bf16x2(f.x * m, f.y * m);
+    for (int k = 0; k < kExpandLoads; ++k) {
+      const int i = i0 + k * kExpandThreads;
+      if (i >= rows * 8) break;
+      const float m = fp8_scale(scale[k]);
+      const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+      uint32_t o[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 f = fp8_to_float2(w[e]), g = fp8_to_float2(w[e] >> 16);
+        o[2 * e] = pack_bf16x2(f.x * m, f.y * m);
+        o[2 * e + 1] = pack_bf16x2(g.x * m, g.y * m);
       }
+      uint4* dst = reinterpret_cast<uint4*>(out + static_cast<size_t>(i) * 16);
+      dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
+      dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
     }
-    uint4* dst = reinterpret_cast<uint4*>(out + i * 16);
-    dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
-    dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
   }
 }
 
@@ -234,7 +259,9 @@ extern "C" int forge_fp8_expand(const void* k_codes, const void* k_scales, const
                                 int* tables, int capacity, unsigned* status, cudaStream_t stream) {
   if (num_seqs <= 0 || table_width <= 0) return 0;
   if (block_size < 1 || num_seqs > 65535) return -1;
-  const int rows = block_size % 64 == 0 ? 64 : block_size;
+  // a CTA's rows: a page's, or a part of them where there are few pages
+  int rows = std::min(block_size, 32 * kExpandLoads);
+  while (rows > 32 && 2ll * capacity * nkv * (block_size / rows) < 4 * device_sm_count()) rows /= 2;
   const long long z = 2ll * nkv * (block_size / rows);
   if (z > 65535) return -1;
   const dim3 grid(static_cast<unsigned>(table_width), static_cast<unsigned>(num_seqs), static_cast<unsigned>(z));

@@ -70,4 +70,4 @@ class Fp8Ops:
         """(``Fp8Rows`` of the normed rows, residual): ``add_rms_norm`` whose normed rows leave in 8 bits, quantised from fp32 per 128 columns.
         ``residual`` is updated in place and returned; without one x is."""
         q, scale = self.C.rms_norm_fp8(x, residual, weight, eps)
-        return Fp8Rows(q, scale, x.dtype), x if residual is None else residual
+        return Fp8Rows.of(q, scale, x.dtype), x if residual is None else residual

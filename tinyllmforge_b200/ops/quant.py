@@ -69,6 +69,13 @@ class Fp8Rows:
             raise ValueError(f"Fp8Rows: scales {tuple(scale.shape)} do not belong to values {tuple(q.shape)}")
         self.q, self.scale, self.dtype = q, scale, dtype
 
+    @classmethod
+    def of(cls, q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype) -> "Fp8Rows":
+        """Of tensors that belong together by their making."""
+        rows = object.__new__(cls)
+        rows.q, rows.scale, rows.dtype = q, scale, dtype
+        return rows
+
     @property
     def shape(self):
         return self.q.shape
