@@ -17,19 +17,25 @@ namespace forge {
 
 // Eight consecutive bf16 values; kVec: one 16-byte access.
 template <bool kVec>
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float v[8]) {
-  if constexpr (kVec) {
-    const uint4 r = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+__device__ __forceinline__ uint4 load8(const __nv_bfloat16* p) {
+  if constexpr (kVec) return *reinterpret_cast<const uint4*>(p);
+  const unsigned short* s = reinterpret_cast<const unsigned short*>(p);
+  return make_uint4(s[0] | static_cast<uint32_t>(s[1]) << 16, s[2] | static_cast<uint32_t>(s[3]) << 16, s[4] | static_cast<uint32_t>(s[5]) << 16,
+                    s[6] | static_cast<uint32_t>(s[7]) << 16);
+}
+__device__ __forceinline__ void unpack8(uint4 r, float v[8]) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[2 * i] = bf16_lo(w[i]);
-      v[2 * i + 1] = bf16_hi(w[i]);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __bfloat162float(p[i]);
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = bf16_lo(w[i]);
+    v[2 * i + 1] = bf16_hi(w[i]);
   }
+}
+// The larger one, NaN if one is.
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
 }
 
 struct Fp8Store {
@@ -48,8 +54,9 @@ struct Fp8Store {
 };
 
 // Eight lanes per head, lane j of them has entries 8j.. and 64 + 8j.., the pairs that the rotation mixes; a warp works on kSets sets of
-// four heads of a token, all of whose loads are under way at once, and fetches position, slot and angles once.  Bound by memory: qkv
-// read once, q and the codes written once.
+// four heads of a token, all of whose loads are under way at once.  Norm weight and rotation make one linear map of a pair, computed once for
+// all query heads and once for all key heads of a token; the root follows it, for keys in the factor that brings entries to codes.
+// Bound by memory: qkv read once, q and the codes written once.
 template <bool kVec, int kSets>
 __global__ void __launch_bounds__(128) fp8_store_kernel(const Fp8Store a) {
   pdl_launch_dependents();
@@ -58,79 +65,104 @@ __global__ void __launch_bounds__(128) fp8_store_kernel(const Fp8Store a) {
   const long long wid = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
   if (wid >= static_cast<long long>(a.T) * groups) return;
   const int lane = threadIdx.x & 31, j = lane & 7, sub = lane >> 3;
+  const unsigned octet = 0xFFu << (8 * sub);             // the lanes of a head; the four heads of a set may be of different kinds
   const int t = static_cast<int>(wid / groups), h0 = static_cast<int>(wid - static_cast<long long>(t) * groups) * 4 * kSets + sub;
-  float lo[kSets][8], hi[kSets][8];
+  uint4 raw[kSets][2];
 #pragma unroll
   for (int k = 0; k < kSets; ++k) {
     const __nv_bfloat16* src = a.qkv + static_cast<size_t>(t) * a.ld + static_cast<size_t>(min(h0 + 4 * k, heads - 1)) * kFp8D + 8 * j;
-    load8<kVec>(src, lo[k]);
-    load8<kVec>(src + 64, hi[k]);
+    raw[k][0] = load8<kVec>(src);
+    raw[k][1] = load8<kVec>(src + 64);
   }
   const long long slot = a.slots[t];
   const bool slot_ok = slot >= 0 && slot < a.num_slots;
   if (slot >= a.num_slots && lane == 0) set_status(a.status, kStatusBadIndex);
-  float c[8], s[8];
-  if (a.rope != nullptr) {
-    const float* cs = a.rope + static_cast<size_t>(min(max(a.positions[t], 0), a.rope_rows - 1)) * kFp8D;
-#pragma unroll
-    for (int i = 0; i < 8; i += 4) {
-      *reinterpret_cast<float4*>(c + i) = *reinterpret_cast<const float4*>(cs + 8 * j + i);
-      *reinterpret_cast<float4*>(s + i) = *reinterpret_cast<const float4*>(cs + 64 + 8 * j + i);
-    }
-  }
+  const long long block = slot / a.block_size;
+  const size_t row0 = static_cast<size_t>(block) * a.nkv * a.block_size + (slot - block * a.block_size);        // of KV head 0
+  const float* cs = a.rope == nullptr ? nullptr : a.rope + static_cast<size_t>(min(max(a.positions[t], 0), a.rope_rows - 1)) * kFp8D + 8 * j;
+
+  float xx[8], xy[8], yx[8], yy[8];                      // x' = x xx - y xy,  y' = y yy + x yx
+  int kind = -1;                                         // 0: for query heads, 1: for key heads
 #pragma unroll
   for (int k = 0; k < kSets; ++k) {
     const int h = h0 + 4 * k;
-    const bool is_q = h < a.nq, is_k = !is_q && h < a.nq + a.nkv;
-    float (&x)[8] = lo[k], (&y)[8] = hi[k];
-    const __nv_bfloat16* w = is_q ? a.qw : is_k ? a.kw : nullptr;
-    float ss = 0.f;
+    if (h >= heads) break;
+    const bool is_q = h < a.nq, is_v = h >= a.nq + a.nkv;
+    float x[8], y[8], inv = 1.f;
+    unpack8(raw[k][0], x);
+    unpack8(raw[k][1], y);
+    if (!is_v) {
+      const __nv_bfloat16* w = is_q ? a.qw : a.kw;
+      if (kind != (is_q ? 0 : 1)) {
+        kind = is_q ? 0 : 1;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss = add_squares(x[i], y[i], ss);
+        for (int i = 0; i < 8; ++i) xx[i] = yy[i] = 1.f;
+        if (w != nullptr) {
+          unpack8(load8<kVec>(w + 8 * j), xx);
+          unpack8(load8<kVec>(w + 64 + 8 * j), yy);
+        }
+        if (cs != nullptr) {
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (w != nullptr) {
-      const float inv = rsqrtf(ss / static_cast<float>(kFp8D) + a.eps);
-      float wl[8], wh[8];
-      load8<kVec>(w + 8 * j, wl);
-      load8<kVec>(w + 64 + 8 * j, wh);
+          for (int i = 0; i < 8; i += 4) {
+            const float4 c = *reinterpret_cast<const float4*>(cs + i), s = *reinterpret_cast<const float4*>(cs + 64 + i);
+            const float cv[4] = {c.x, c.y, c.z, c.w}, sv[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              yx[i + e] = xx[i + e] * sv[e];
+              xy[i + e] = yy[i + e] * sv[e];
+              xx[i + e] *= cv[e];
+              yy[i + e] *= cv[e];
+            }
+          }
+        }
+      }
+      if (w != nullptr) {
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], fmaf(y[i], y[i], ss));
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) ss += __shfl_xor_sync(octet, ss, o);
+        inv = rsqrtf(ss * (1.f / kFp8D) + a.eps);
+      }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        x[i] = x[i] * inv * wl[i];
-        y[i] = y[i] * inv * wh[i];
+        const float u = x[i] * xx[i], v = y[i] * yy[i];
+        if (cs != nullptr) {
+          const float x0 = x[i];
+          x[i] = fmaf(-y[i], xy[i], u);
+          y[i] = fmaf(x0, yx[i], v);
+        } else {
+          x[i] = u;
+          y[i] = v;
+        }
       }
     }
-    if (a.rope != nullptr && (is_q || is_k)) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) rotate_pair(x[i], y[i], c[i], s[i]);
-    }
-    uint32_t amax = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) amax = max(amax, max(abs_bits(x[i]), abs_bits(y[i])));
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    if (h >= heads) continue;
     if (is_q) {
       __nv_bfloat16* dst = a.q_out + (static_cast<size_t>(t) * a.nq + h) * kFp8D + 8 * j;
-      *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
-      *reinterpret_cast<uint4*>(dst + 64) = make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7]));
+      *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16x2(x[0] * inv, x[1] * inv), pack_bf16x2(x[2] * inv, x[3] * inv), pack_bf16x2(x[4] * inv, x[5] * inv),
+                                                  pack_bf16x2(x[6] * inv, x[7] * inv));
+      *reinterpret_cast<uint4*>(dst + 64) = make_uint4(pack_bf16x2(y[0] * inv, y[1] * inv), pack_bf16x2(y[2] * inv, y[3] * inv),
+                                                       pack_bf16x2(y[4] * inv, y[5] * inv), pack_bf16x2(y[6] * inv, y[7] * inv));
       continue;
     }
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) amax = max_or_nan(amax, max_or_nan(fabsf(x[i]), fabsf(y[i])));
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) amax = max_or_nan(amax, __shfl_xor_sync(octet, amax, o));
     if (!slot_ok) continue;
-    const int kvh = is_k ? h - a.nq : h - a.nq - a.nkv;
-    const long long block = slot / a.block_size;
-    const size_t row = (static_cast<size_t>(block) * a.nkv + kvh) * a.block_size + (slot - block * a.block_size);
-    const uint32_t b = fp8_scale_byte(amax);
+    const size_t row = row0 + static_cast<size_t>(is_v ? h - a.nq - a.nkv : h - a.nq) * a.block_size;
+    const uint32_t b = fp8_scale_byte(abs_bits(amax * inv));
     uint2 code[2] = {make_uint2(kCodesNan, kCodesNan), make_uint2(kCodesNan, kCodesNan)};
     if (b != kScaleNan) {
-      const float m = fp8_inverse_scale(b);
+      const float m = fp8_inverse_scale(b) * inv;
       code[0] = make_uint2(fp8_pack(x[0] * m, x[1] * m, x[2] * m, x[3] * m), fp8_pack(x[4] * m, x[5] * m, x[6] * m, x[7] * m));
       code[1] = make_uint2(fp8_pack(y[0] * m, y[1] * m, y[2] * m, y[3] * m), fp8_pack(y[4] * m, y[5] * m, y[6] * m, y[7] * m));
     }
-    uint8_t* dst = (is_k ? a.k_codes : a.v_codes) + row * kFp8D + 8 * j;
+    uint8_t* dst = (is_v ? a.v_codes : a.k_codes) + row * kFp8D + 8 * j;
     *reinterpret_cast<uint2*>(dst) = code[0];
     *reinterpret_cast<uint2*>(dst + 64) = code[1];
-    if (j == 0) (is_k ? a.k_scales : a.v_scales)[row] = static_cast<uint8_t>(b);
+    if (j == 0) (is_v ? a.v_scales : a.k_scales)[row] = static_cast<uint8_t>(b);
   }
 }
 
@@ -158,7 +190,7 @@ extern "C" int forge_fp8_store(const void* qkv, long long ld, const void* qw, co
   auto aligned = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
   const bool vec = ld % 8 == 0 && aligned(qkv) && aligned(qw) && aligned(kw);
   if (!vec) return launch_store<false, 1>(a, stream);
-  return T < 512 ? launch_store<true, 1>(a, stream) : launch_store<true, 2>(a, stream);
+  return T < 512 ? launch_store<true, 1>(a, stream) : T < 2048 ? launch_store<true, 2>(a, stream) : launch_store<true, 4>(a, stream);
 }
 
 // ---------------------------------------------------------------------------------------------------------

@@ -3,10 +3,11 @@
 //   s = x + r, rounded to bf16 and stored in r;   y = s w / sqrt(mean(s^2) + eps), in fp32
 //   per 128 entries:  scale = max|y| / 448 (1 where all are zero),  codes = e4m3(y / scale)
 //
-// Few rows: one CTA per row, a thread has eight entries (16 threads a group of 128).  Many rows: one warp per row, all of its loads under
-// way at once and no barrier; the row stays in registers as the bf16 it is held in.  Bound by memory: 7 bytes per entry with a residual, 3
-// without, where a norm and a quantiser of their own move 10 (6) and need two launches.  The norm is not rounded before it is
-// quantised.  No counterpart in the reference.
+// The root is a factor of every entry and of the largest one, so the codes do not depend on it: with t = s w they are e4m3(t m), m = 448 / max|t|, and
+// scale = 1 / (m sqrt(mean(s^2) + eps)).  Entries therefore go from load to store in one pass and no row waits for its sum; only
+// the scales, one for 128 entries, are written after it.  One CTA per row, a thread has eight entries, 16 threads a group of 128.
+// Bound by memory: 7 bytes per entry with a residual, 3 without, where a norm and a quantiser of their own move 10 (6) and need two
+// launches.  The norm is not rounded before it is quantised.  No counterpart in the reference.
 #include "../include/fp8_cache.cuh"
 #include "../include/launch.cuh"
 #include "../include/ptx.cuh"
@@ -14,7 +15,7 @@
 
 namespace forge {
 
-constexpr int kNormFp8Threads = 512;
+constexpr int kNormFp8Threads = 1024;
 
 struct NormFp8 {
   const __nv_bfloat16* x;
@@ -22,48 +23,11 @@ struct NormFp8 {
   const __nv_bfloat16* w;
   uint8_t* codes;
   float* scales;
-  int scale_ld, rows, H;
+  int scale_ld, H;
   float eps;
 };
 
-// Eight entries of the stream as four pairs of bf16: x, or x + r rounded and stored; adds their squares.
-template <bool kAdd>
-__device__ __forceinline__ uint4 norm_fp8_take(uint4 v, uint4 r, __nv_bfloat16* to, float& ss) {
-  uint32_t s[4] = {v.x, v.y, v.z, v.w};
-  if constexpr (kAdd) {
-    const uint32_t b[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s[i] = pack_bf16x2(bf16_lo(s[i]) + bf16_lo(b[i]), bf16_hi(s[i]) + bf16_hi(b[i]));
-    *reinterpret_cast<uint4*>(to) = make_uint4(s[0], s[1], s[2], s[3]);
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) ss = fmaf(bf16_lo(s[i]), bf16_lo(s[i]), fmaf(bf16_hi(s[i]), bf16_hi(s[i]), ss));
-  return make_uint4(s[0], s[1], s[2], s[3]);
-}
-
-// Vector i of a row (entries 8 i ..) normed and quantised; 16 neighbouring lanes have a group and come here together.  `in`: there is such a vector.
-__device__ __forceinline__ void norm_fp8_put(const NormFp8& a, size_t row, int i, bool in, uint4 s, float inv) {
-  float y[8], amax = 0.f;
-  if (in) {
-    const uint4 wv = *reinterpret_cast<const uint4*>(a.w + 8 * i);
-    const uint32_t v[4] = {s.x, s.y, s.z, s.w}, w[4] = {wv.x, wv.y, wv.z, wv.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      y[2 * e] = bf16_lo(v[e]) * inv * bf16_lo(w[e]);
-      y[2 * e + 1] = bf16_hi(v[e]) * inv * bf16_hi(w[e]);
-      amax = fmaxf(amax, fmaxf(fabsf(y[2 * e]), fabsf(y[2 * e + 1])));
-    }
-  }
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  if (!in) return;
-  const float scale = amax > 0.f ? amax / 448.f : 1.f, m = 1.f / scale;
-  *reinterpret_cast<uint2*>(a.codes + row * a.H + 8 * i) =
-      make_uint2(fp8_pack(y[0] * m, y[1] * m, y[2] * m, y[3] * m), fp8_pack(y[4] * m, y[5] * m, y[6] * m, y[7] * m));
-  if ((i & 15) == 0) a.scales[static_cast<size_t>(i >> 4) * a.scale_ld + row] = scale;
-}
-
-// One CTA per row; kVectors of eight entries per thread.
+// kVectors of eight entries per thread.
 template <bool kAdd, int kVectors>
 __global__ void __launch_bounds__(kNormFp8Threads) rms_norm_fp8_kernel(const NormFp8 a) {
   __shared__ float red[kNormFp8Threads / 32];
@@ -71,85 +35,71 @@ __global__ void __launch_bounds__(kNormFp8Threads) rms_norm_fp8_kernel(const Nor
   pdl_wait();
   const size_t row = blockIdx.x;
   const int nvec = a.H >> 3, warps = blockDim.x >> 5;
-  uint4 s[kVectors];
-  float ss = 0.f;
+  float m[kVectors], ss = 0.f;                          // m: 0 for a group of zeros
 #pragma unroll
   for (int c = 0; c < kVectors; ++c) {
     const int i = threadIdx.x + c * blockDim.x;
+    m[c] = 0.f;
+    if (c * static_cast<int>(blockDim.x) >= nvec) break;             // uniform: the shuffles below take whole warps
+    float t[8], amax = 0.f;
+    if (i < nvec) {
+      const size_t at = row * a.H + 8 * i;
+      const uint4 xv = *reinterpret_cast<const uint4*>(a.x + at), wv = *reinterpret_cast<const uint4*>(a.w + 8 * i);
+      uint32_t s[4] = {xv.x, xv.y, xv.z, xv.w};
+      const uint32_t w[4] = {wv.x, wv.y, wv.z, wv.w};
+      if constexpr (kAdd) {
+        const uint4 rv = *reinterpret_cast<const uint4*>(a.residual + at);
+        const uint32_t r[4] = {rv.x, rv.y, rv.z, rv.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] = pack_bf16x2(bf16_lo(s[e]) + bf16_lo(r[e]), bf16_hi(s[e]) + bf16_hi(r[e]));
+        *reinterpret_cast<uint4*>(a.residual + at) = make_uint4(s[0], s[1], s[2], s[3]);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float lo = bf16_lo(s[e]), hi = bf16_hi(s[e]);
+        ss = fmaf(lo, lo, fmaf(hi, hi, ss));
+        t[2 * e] = lo * bf16_lo(w[e]);
+        t[2 * e + 1] = hi * bf16_hi(w[e]);
+        amax = fmaxf(amax, fmaxf(fabsf(t[2 * e]), fabsf(t[2 * e + 1])));
+      }
+    }
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
     if (i >= nvec) continue;
-    const size_t at = row * a.H + 8 * i;
-    s[c] = norm_fp8_take<kAdd>(*reinterpret_cast<const uint4*>(a.x + at), kAdd ? *reinterpret_cast<const uint4*>(a.residual + at) : make_uint4(0, 0, 0, 0),
-                               a.residual + at, ss);
+    const float mul = fminf(448.f / amax, 0x1p126f);    // (infinite for zeros and for what is next to them)
+    *reinterpret_cast<uint2*>(a.codes + row * a.H + 8 * i) =
+        make_uint2(fp8_pack(t[0] * mul, t[1] * mul, t[2] * mul, t[3] * mul), fp8_pack(t[4] * mul, t[5] * mul, t[6] * mul, t[7] * mul));
+    m[c] = amax == 0.f ? 0.f : mul;
   }
   ss = warp_sum_f(ss);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = ss;
   __syncthreads();
+  if (threadIdx.x & 15) return;
   ss = 0.f;
   for (int i = 0; i < warps; ++i) ss += red[i];
   const float inv = rsqrtf(ss / static_cast<float>(a.H) + a.eps);
 #pragma unroll
   for (int c = 0; c < kVectors; ++c) {
     const int i = threadIdx.x + c * blockDim.x;
-    if (c * static_cast<int>(blockDim.x) < nvec) norm_fp8_put(a, row, i, i < nvec, s[c], inv);           // (uniform: whole warps)
+    if (i < nvec) a.scales[static_cast<size_t>(i >> 4) * a.scale_ld + row] = m[c] != 0.f ? inv / m[c] : inv == inv ? 1.f : inv;   // (NaN in the row)
   }
-}
-
-// One warp per row; kVectors of eight entries per lane.
-template <bool kAdd, int kVectors>
-__global__ void __launch_bounds__(128) rms_norm_fp8_warp_kernel(const NormFp8 a) {
-  pdl_launch_dependents();
-  pdl_wait();
-  const int lane = threadIdx.x & 31, nvec = a.H >> 3;
-  const size_t row = static_cast<size_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (row >= static_cast<size_t>(a.rows)) return;
-  uint4 s[kVectors], r[kAdd ? kVectors : 1];
-#pragma unroll
-  for (int c = 0; c < kVectors; ++c) {
-    const int i = lane + 32 * c;
-    if (i >= nvec) continue;
-    s[c] = *reinterpret_cast<const uint4*>(a.x + row * a.H + 8 * i);
-    if constexpr (kAdd) r[c] = *reinterpret_cast<const uint4*>(a.residual + row * a.H + 8 * i);
-  }
-  float ss = 0.f;
-#pragma unroll
-  for (int c = 0; c < kVectors; ++c) {
-    const int i = lane + 32 * c;
-    if (i < nvec) s[c] = norm_fp8_take<kAdd>(s[c], r[kAdd ? c : 0], a.residual + row * a.H + 8 * i, ss);
-  }
-  const float inv = rsqrtf(warp_sum_f(ss) / static_cast<float>(a.H) + a.eps);
-#pragma unroll
-  for (int c = 0; c < kVectors; ++c)
-    if (32 * c < nvec) norm_fp8_put(a, row, lane + 32 * c, lane + 32 * c < nvec, s[c], inv);
 }
 
 template <int kVectors>
-static cudaError_t launch_rows(const NormFp8& a, cudaStream_t stream) {
-  int threads = ((a.H >> 3) + 31) / 32 * 32;
-  if (threads > kNormFp8Threads) threads = kNormFp8Threads;
-  return launch_kernel(a.residual != nullptr ? rms_norm_fp8_kernel<true, kVectors> : rms_norm_fp8_kernel<false, kVectors>, dim3(a.rows), dim3(threads), 0,
+static cudaError_t launch_rows(const NormFp8& a, int rows, cudaStream_t stream) {
+  const int threads = ((a.H / 8 + kVectors - 1) / kVectors + 31) / 32 * 32;
+  return launch_kernel(a.residual != nullptr ? rms_norm_fp8_kernel<true, kVectors> : rms_norm_fp8_kernel<false, kVectors>, dim3(rows), dim3(threads), 0,
                        stream, 0, a);
-}
-template <int kVectors>
-static cudaError_t launch_warps(const NormFp8& a, cudaStream_t stream) {
-  return launch_kernel(a.residual != nullptr ? rms_norm_fp8_warp_kernel<true, kVectors> : rms_norm_fp8_warp_kernel<false, kVectors>, dim3((a.rows + 3) / 4),
-                       dim3(128), 0, stream, 0, a);
 }
 
 // x, residual [rows][H] bf16 (residual may be null), w [H], codes [rows][H], scales [H / 128][scale_ld >= rows].
 extern "C" int forge_rms_norm_fp8(const void* x, void* residual, const void* w, void* codes, float* scales, int scale_ld, int rows, int H,
                                   float eps, cudaStream_t stream) {
   if (rows <= 0) return 0;
-  if (H < 128 || H % 128 != 0 || H > 4 * kNormFp8Threads * 8 || scale_ld < rows) return -1;
+  if (H < 128 || H % 128 != 0 || H > 2 * kNormFp8Threads * 8 || scale_ld < rows) return -1;
   const NormFp8 a{static_cast<const __nv_bfloat16*>(x), static_cast<__nv_bfloat16*>(residual), static_cast<const __nv_bfloat16*>(w),
-                  static_cast<uint8_t*>(codes), scales, scale_ld, rows, H, eps};
-  cudaError_t e;
-  if (rows < 8 * device_sm_count() || H > 5120) e = H <= kNormFp8Threads * 8 ? launch_rows<1>(a, stream) : launch_rows<4>(a, stream);
-  else if (H <= 1024) e = launch_warps<4>(a, stream);
-  else if (H <= 2048) e = launch_warps<8>(a, stream);
-  else if (H <= 2560) e = launch_warps<10>(a, stream);
-  else if (H <= 4096) e = launch_warps<16>(a, stream);
-  else e = launch_warps<20>(a, stream);
-  return e == cudaSuccess ? 0 : -2;
+                  static_cast<uint8_t*>(codes), scales, scale_ld, H, eps};
+  return (H <= kNormFp8Threads * 8 ? launch_rows<1>(a, rows, stream) : launch_rows<2>(a, rows, stream)) == cudaSuccess ? 0 : -2;
 }
 
 }  // namespace forge
