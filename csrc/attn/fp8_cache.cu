@@ -48,129 +48,181 @@ struct Fp8Store {
   const int *positions, *slots;
   __nv_bfloat16* q_out;
   uint8_t *k_codes, *k_scales, *v_codes, *v_scales;
-  int T, nq, nkv, block_size;
-  long long num_slots;
+  int T, nq, nkv, block_size, num_slots;
   unsigned* status;
 };
 
-// Eight lanes per head, lane j of them has entries 8j.. and 64 + 8j.., the pairs that the rotation mixes; a warp works on kSets sets of
-// four heads of a token, all of whose loads are under way at once.  Norm weight and rotation make one linear map of a pair, computed once for
-// all query heads and once for all key heads of a token; the root follows it, for keys in the factor that brings entries to codes.
-// Bound by memory: qkv read once, q and the codes written once.
-template <bool kVec, int kSets>
+// Eight lanes per head, lane j of them has entries 8j.. and 64 + 8j.., the pairs that the rotation mixes; a warp has a set of four heads.  raw: the
+// head's entries; cs: cos and sin of the token at 8j and 64 + 8j, null: no rotation; row0: the slot's row of KV head 0.
+template <bool kVec>
+__device__ __forceinline__ void fp8_store_head(const Fp8Store& a, int t, int h, const uint4* raw, const float* cs, bool slot_ok, size_t row0, int lane) {
+  const int j = lane & 7;
+  const unsigned octet = 0xFFu << (lane & 24);           // the lanes of a head; the four heads of a set may be of different kinds
+  const bool is_q = h < a.nq, is_v = h >= a.nq + a.nkv;
+  float x[8], y[8], inv = 1.f;
+  unpack8(raw[0], x);
+  unpack8(raw[1], y);
+  if (!is_v) {
+    const __nv_bfloat16* w = is_q ? a.qw : a.kw;
+    if (w != nullptr) {                                  // the root is a factor of all entries and comes last
+      const uint4 wl = load8<kVec>(w + 8 * j), wh = load8<kVec>(w + 64 + 8 * j);
+      float ss = 0.f, v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], fmaf(y[i], y[i], ss));
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) ss += __shfl_xor_sync(octet, ss, o);
+      inv = rsqrtf(ss * (1.f / kFp8D) + a.eps);
+      unpack8(wl, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] *= v[i];
+      unpack8(wh, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] *= v[i];
+    }
+    if (cs != nullptr) {
+#pragma unroll
+      for (int i = 0; i < 8; i += 4) {
+        const float4 c = *reinterpret_cast<const float4*>(cs + i), s = *reinterpret_cast<const float4*>(cs + 64 + i);
+        rotate_pair(x[i], y[i], c.x, s.x);
+        rotate_pair(x[i + 1], y[i + 1], c.y, s.y);
+        rotate_pair(x[i + 2], y[i + 2], c.z, s.z);
+        rotate_pair(x[i + 3], y[i + 3], c.w, s.w);
+      }
+    }
+  }
+  if (is_q) {
+    __nv_bfloat16* dst = a.q_out + (static_cast<size_t>(t) * a.nq + h) * kFp8D + 8 * j;
+    *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16x2(x[0] * inv, x[1] * inv), pack_bf16x2(x[2] * inv, x[3] * inv), pack_bf16x2(x[4] * inv, x[5] * inv),
+                                                pack_bf16x2(x[6] * inv, x[7] * inv));
+    *reinterpret_cast<uint4*>(dst + 64) = make_uint4(pack_bf16x2(y[0] * inv, y[1] * inv), pack_bf16x2(y[2] * inv, y[3] * inv),
+                                                     pack_bf16x2(y[4] * inv, y[5] * inv), pack_bf16x2(y[6] * inv, y[7] * inv));
+    return;
+  }
+  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) amax = max_or_nan(amax, max_or_nan(fabsf(x[i]), fabsf(y[i])));
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) amax = max_or_nan(amax, __shfl_xor_sync(octet, amax, o));
+  if (!slot_ok) return;
+  const size_t row = row0 + static_cast<size_t>(is_v ? h - a.nq - a.nkv : h - a.nq) * a.block_size;
+  const uint32_t b = fp8_scale_byte(abs_bits(amax * inv));
+  uint2 code[2] = {make_uint2(kCodesNan, kCodesNan), make_uint2(kCodesNan, kCodesNan)};
+  if (b != kScaleNan) {
+    const float m = fp8_inverse_scale(b);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x[i] = x[i] * inv * m;
+      y[i] = y[i] * inv * m;
+    }
+    code[0] = make_uint2(fp8_pack(x[0], x[1], x[2], x[3]), fp8_pack(x[4], x[5], x[6], x[7]));
+    code[1] = make_uint2(fp8_pack(y[0], y[1], y[2], y[3]), fp8_pack(y[4], y[5], y[6], y[7]));
+  }
+  uint8_t* dst = (is_v ? a.v_codes : a.k_codes) + row * kFp8D + 8 * j;
+  *reinterpret_cast<uint2*>(dst) = code[0];
+  *reinterpret_cast<uint2*>(dst + 64) = code[1];
+  if (j == 0) (is_v ? a.v_scales : a.k_scales)[row] = static_cast<uint8_t>(b);
+}
+
+// The slot's row of KV head 0; false: no such slot, or none.
+__device__ __forceinline__ bool fp8_slot_row(const Fp8Store& a, int slot, size_t& row0) {
+  const int block = slot / a.block_size;
+  row0 = static_cast<size_t>(block) * a.nkv * a.block_size + (slot - block * a.block_size);
+  return slot >= 0 && slot < a.num_slots;
+}
+__device__ __forceinline__ int fp8_angle_row(const Fp8Store& a, int position) { return min(max(position, 0), a.rope_rows - 1); }
+
+// Few tokens, or rows that are not aligned: a warp per set of heads.
+template <bool kVec>
 __global__ void __launch_bounds__(128) fp8_store_kernel(const Fp8Store a) {
   pdl_launch_dependents();
   pdl_wait();
-  const int heads = a.nq + 2 * a.nkv, groups = (heads + 4 * kSets - 1) / (4 * kSets);
+  const int heads = a.nq + 2 * a.nkv, sets = (heads + 3) / 4;
   const long long wid = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (wid >= static_cast<long long>(a.T) * groups) return;
-  const int lane = threadIdx.x & 31, j = lane & 7, sub = lane >> 3;
-  const unsigned octet = 0xFFu << (8 * sub);             // the lanes of a head; the four heads of a set may be of different kinds
-  const int t = static_cast<int>(wid / groups), h0 = static_cast<int>(wid - static_cast<long long>(t) * groups) * 4 * kSets + sub;
-  uint4 raw[kSets][2];
-#pragma unroll
-  for (int k = 0; k < kSets; ++k) {
-    const __nv_bfloat16* src = a.qkv + static_cast<size_t>(t) * a.ld + static_cast<size_t>(min(h0 + 4 * k, heads - 1)) * kFp8D + 8 * j;
-    raw[k][0] = load8<kVec>(src);
-    raw[k][1] = load8<kVec>(src + 64);
-  }
-  const long long slot = a.slots[t];
-  const bool slot_ok = slot >= 0 && slot < a.num_slots;
+  if (wid >= static_cast<long long>(a.T) * sets) return;
+  const int lane = threadIdx.x & 31, j = lane & 7;
+  const int t = static_cast<int>(wid / sets), h = static_cast<int>(wid - static_cast<long long>(t) * sets) * 4 + (lane >> 3);
+  const __nv_bfloat16* src = a.qkv + static_cast<size_t>(t) * a.ld + static_cast<size_t>(min(h, heads - 1)) * kFp8D + 8 * j;
+  const uint4 raw[2] = {load8<kVec>(src), load8<kVec>(src + 64)};
+  const int slot = a.slots[t];
   if (slot >= a.num_slots && lane == 0) set_status(a.status, kStatusBadIndex);
-  const long long block = slot / a.block_size;
-  const size_t row0 = static_cast<size_t>(block) * a.nkv * a.block_size + (slot - block * a.block_size);        // of KV head 0
-  const float* cs = a.rope == nullptr ? nullptr : a.rope + static_cast<size_t>(min(max(a.positions[t], 0), a.rope_rows - 1)) * kFp8D + 8 * j;
-
-  float xx[8], xy[8], yx[8], yy[8];                      // x' = x xx - y xy,  y' = y yy + x yx
-  int kind = -1;                                         // 0: for query heads, 1: for key heads
-#pragma unroll
-  for (int k = 0; k < kSets; ++k) {
-    const int h = h0 + 4 * k;
-    if (h >= heads) break;
-    const bool is_q = h < a.nq, is_v = h >= a.nq + a.nkv;
-    float x[8], y[8], inv = 1.f;
-    unpack8(raw[k][0], x);
-    unpack8(raw[k][1], y);
-    if (!is_v) {
-      const __nv_bfloat16* w = is_q ? a.qw : a.kw;
-      if (kind != (is_q ? 0 : 1)) {
-        kind = is_q ? 0 : 1;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) xx[i] = yy[i] = 1.f;
-        if (w != nullptr) {
-          unpack8(load8<kVec>(w + 8 * j), xx);
-          unpack8(load8<kVec>(w + 64 + 8 * j), yy);
-        }
-        if (cs != nullptr) {
-#pragma unroll
-          for (int i = 0; i < 8; i += 4) {
-            const float4 c = *reinterpret_cast<const float4*>(cs + i), s = *reinterpret_cast<const float4*>(cs + 64 + i);
-            const float cv[4] = {c.x, c.y, c.z, c.w}, sv[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              yx[i + e] = xx[i + e] * sv[e];
-              xy[i + e] = yy[i + e] * sv[e];
-              xx[i + e] *= cv[e];
-              yy[i + e] *= cv[e];
-            }
-          }
-        }
-      }
-      if (w != nullptr) {
-        float ss = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], fmaf(y[i], y[i], ss));
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) ss += __shfl_xor_sync(octet, ss, o);
-        inv = rsqrtf(ss * (1.f / kFp8D) + a.eps);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float u = x[i] * xx[i], v = y[i] * yy[i];
-        if (cs != nullptr) {
-          const float x0 = x[i];
-          x[i] = fmaf(-y[i], xy[i], u);
-          y[i] = fmaf(x0, yx[i], v);
-        } else {
-          x[i] = u;
-          y[i] = v;
-        }
-      }
-    }
-    if (is_q) {
-      __nv_bfloat16* dst = a.q_out + (static_cast<size_t>(t) * a.nq + h) * kFp8D + 8 * j;
-      *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16x2(x[0] * inv, x[1] * inv), pack_bf16x2(x[2] * inv, x[3] * inv), pack_bf16x2(x[4] * inv, x[5] * inv),
-                                                  pack_bf16x2(x[6] * inv, x[7] * inv));
-      *reinterpret_cast<uint4*>(dst + 64) = make_uint4(pack_bf16x2(y[0] * inv, y[1] * inv), pack_bf16x2(y[2] * inv, y[3] * inv),
-                                                       pack_bf16x2(y[4] * inv, y[5] * inv), pack_bf16x2(y[6] * inv, y[7] * inv));
-      continue;
-    }
-    float amax = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) amax = max_or_nan(amax, max_or_nan(fabsf(x[i]), fabsf(y[i])));
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) amax = max_or_nan(amax, __shfl_xor_sync(octet, amax, o));
-    if (!slot_ok) continue;
-    const size_t row = row0 + static_cast<size_t>(is_v ? h - a.nq - a.nkv : h - a.nq) * a.block_size;
-    const uint32_t b = fp8_scale_byte(abs_bits(amax * inv));
-    uint2 code[2] = {make_uint2(kCodesNan, kCodesNan), make_uint2(kCodesNan, kCodesNan)};
-    if (b != kScaleNan) {
-      const float m = fp8_inverse_scale(b) * inv;
-      code[0] = make_uint2(fp8_pack(x[0] * m, x[1] * m, x[2] * m, x[3] * m), fp8_pack(x[4] * m, x[5] * m, x[6] * m, x[7] * m));
-      code[1] = make_uint2(fp8_pack(y[0] * m, y[1] * m, y[2] * m, y[3] * m), fp8_pack(y[4] * m, y[5] * m, y[6] * m, y[7] * m));
-    }
-    uint8_t* dst = (is_v ? a.v_codes : a.k_codes) + row * kFp8D + 8 * j;
-    *reinterpret_cast<uint2*>(dst) = code[0];
-    *reinterpret_cast<uint2*>(dst + 64) = code[1];
-    if (j == 0) (is_v ? a.v_scales : a.k_scales)[row] = static_cast<uint8_t>(b);
-  }
+  size_t row0;
+  const bool slot_ok = fp8_slot_row(a, slot, row0);
+  const float* cs = a.rope == nullptr ? nullptr : a.rope + static_cast<size_t>(fp8_angle_row(a, a.positions[t])) * kFp8D + 8 * j;
+  if (h < heads) fp8_store_head<kVec>(a, t, h, raw, cs, slot_ok, row0, lane);
 }
 
-template <bool kVec, int kSets>
-static int launch_store(const Fp8Store& a, cudaStream_t stream) {
-  const int groups = (a.nq + 2 * a.nkv + 4 * kSets - 1) / (4 * kSets);
-  const dim3 grid(static_cast<unsigned>((static_cast<long long>(a.T) * groups + 3) / 4));
-  return launch_kernel(fp8_store_kernel<kVec, kSets>, grid, dim3(128), 0, stream, 0, a) == cudaSuccess ? 0 : -2;
+// Many tokens: a loading warp brings whole rows of the projection and their angles into a ring by bulk copies, the others take sets of heads
+// from it, so that memory is asked ahead of the arithmetic whatever that takes.  Persistent, two CTAs per SM; shared memory is asked for
+// so that no third fits beside them: of equal shares none may wait for a CTA that another SM would have had room for.
+constexpr int kStoreRing = 1024;                       // tokens from which on
+constexpr int kStoreWarps = 12, kStoreCtasPerSm = 2, kStoreSmem = 108 * 1024, kStoreMaxStages = 8;
+
+__global__ void __launch_bounds__(32 * (kStoreWarps + 1), kStoreCtasPerSm) fp8_store_ring_kernel(const Fp8Store a, int stages) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint64_t full[kStoreMaxStages], empty[kStoreMaxStages];
+  __shared__ int s_slot[kStoreMaxStages];
+  const int heads = a.nq + 2 * a.nkv, sets = (heads + 3) / 4, row_bytes = heads * kFp8D * 2, stage_bytes = row_bytes + kFp8D * 4;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, consumers = (blockDim.x >> 5) - 1;
+  pdl_launch_dependents();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], consumers);
+    }
+    fence_mbar_init();
+  }
+  __syncthreads();
+  pdl_wait();
+  int s = 0, phase = 0;
+  const auto next = [&] {
+    if (++s == stages) {
+      s = 0;
+      phase ^= 1;
+    }
+  };
+  if (warp == consumers) {
+    bool ok = true;
+    for (int t0 = blockIdx.x; t0 < a.T && ok; t0 += 32 * gridDim.x) {             // slots and positions of 32 tokens at a time
+      const int mine = t0 + lane * gridDim.x;
+      const int slot = mine < a.T ? a.slots[mine] : -1, at = mine < a.T && a.rope != nullptr ? fp8_angle_row(a, a.positions[mine]) : 0;
+      if (slot >= a.num_slots) set_status(a.status, kStatusBadIndex);
+      for (int i = 0; i < 32 && ok; ++i) {
+        const int t = t0 + i * gridDim.x, to = __shfl_sync(0xffffffffu, slot, i), angle = __shfl_sync(0xffffffffu, at, i);
+        if (t >= a.T) break;
+        if (lane == 0) {
+          ok = mbar_wait_parked(&empty[s], phase ^ 1, a.status);
+          if (ok) {
+            uint8_t* stage = smem + s * stage_bytes;
+            s_slot[s] = to;
+            mbar_expect_tx(&full[s], a.rope != nullptr ? stage_bytes : row_bytes);
+            bulk_load(stage, a.qkv + static_cast<size_t>(t) * a.ld, row_bytes, &full[s]);
+            if (a.rope != nullptr) bulk_load(stage + row_bytes, a.rope + static_cast<size_t>(angle) * kFp8D, kFp8D * 4, &full[s]);
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        next();
+      }
+    }
+    return;
+  }
+  const int j = lane & 7;
+  for (int t = blockIdx.x; t < a.T; t += gridDim.x, next()) {
+    if (!mbar_wait(&full[s], phase, a.status)) return;
+    const uint8_t* stage = smem + s * stage_bytes;
+    size_t row0;
+    const bool slot_ok = fp8_slot_row(a, s_slot[s], row0);
+    const float* cs = a.rope == nullptr ? nullptr : reinterpret_cast<const float*>(stage + row_bytes) + 8 * j;
+    for (int set = warp; set < sets; set += consumers) {
+      const int h = 4 * set + (lane >> 3);
+      if (h < heads) {
+        const uint4* src = reinterpret_cast<const uint4*>(stage + h * kFp8D * 2) + j;
+        const uint4 raw[2] = {src[0], src[8]};
+        fp8_store_head<true>(a, t, h, raw, cs, slot_ok, row0, lane);
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&empty[s]);
+  }
 }
 
 // qkv [T, (nq + 2 nkv) * 128] with rows ld apart; rope fp32 [rope_rows][128] = cos, sin; slot < 0 is passed over, slot >= num_slots too and
@@ -186,18 +238,26 @@ extern "C" int forge_fp8_store(const void* qkv, long long ld, const void* qw, co
   a.q_out = static_cast<__nv_bfloat16*>(q_out);
   a.k_codes = static_cast<uint8_t*>(k_codes); a.k_scales = static_cast<uint8_t*>(k_scales);
   a.v_codes = static_cast<uint8_t*>(v_codes); a.v_scales = static_cast<uint8_t*>(v_scales);
-  a.T = T; a.nq = nq; a.nkv = nkv; a.block_size = block_size; a.num_slots = num_slots; a.status = status;
-  auto aligned = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+  a.T = T; a.nq = nq; a.nkv = nkv; a.block_size = block_size; a.num_slots = static_cast<int>(num_slots); a.status = status;
+  const auto aligned = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
   const bool vec = ld % 8 == 0 && aligned(qkv) && aligned(qw) && aligned(kw);
-  if (!vec) return launch_store<false, 1>(a, stream);
-  return T < 512 ? launch_store<true, 1>(a, stream) : T < 2048 ? launch_store<true, 2>(a, stream) : launch_store<true, 4>(a, stream);
+  const int heads = nq + 2 * nkv, sets = (heads + 3) / 4, stage = heads * kFp8D * 2 + kFp8D * 4;
+  const int stages = std::min(kStoreMaxStages, kStoreSmem / stage);
+  if (vec && stages >= 3 && T >= kStoreRing) {
+    FORGE_ENSURE_DYN_SMEM(fp8_store_ring_kernel, kStoreSmem);
+    const int ctas = std::min(T, kStoreCtasPerSm * device_sm_count());
+    return launch_kernel(fp8_store_ring_kernel, dim3(ctas), dim3(32 * (std::min(sets, kStoreWarps) + 1)), kStoreSmem, stream, 0, a, stages) == cudaSuccess
+               ? 0 : -2;
+  }
+  const dim3 grid(static_cast<unsigned>((static_cast<long long>(T) * sets + 3) / 4));
+  return launch_kernel(vec ? fp8_store_kernel<true> : fp8_store_kernel<false>, grid, dim3(128), 0, stream, 0, a) == cudaSuccess ? 0 : -2;
 }
 
 // ---------------------------------------------------------------------------------------------------------
 // Pages of sequences, in order, as bf16.  A CTA takes `rows` token rows of one page of one head of K or V.  Lengths, table entry and, once the
 // latter is there, the codes are asked for one after the other; where the page goes is found out meanwhile.  Bound by memory.
 // ---------------------------------------------------------------------------------------------------------
-constexpr int kExpandThreads = 256, kExpandLoads = 4;
+constexpr int kExpandThreads = 256, kExpandLoads = 8;
 
 __global__ void __launch_bounds__(kExpandThreads) fp8_expand_kernel(
     const uint8_t* __restrict__ k_codes, const uint8_t* __restrict__ k_scales, const uint8_t* __restrict__ v_codes,
@@ -233,15 +293,15 @@ __global__ void __launch_bounds__(kExpandThreads) fp8_expand_kernel(
   const int live = min(len - page * block_size - part * rows, rows);
   const uint8_t* codes = (is_v ? v_codes : k_codes) + row0 * kFp8D;
   const uint8_t* scales = (is_v ? v_scales : k_scales) + row0;
-  uint4 raw[kExpandLoads];
+  uint2 raw[kExpandLoads];
   uint32_t scale[kExpandLoads];
-  const auto fetch = [&](int i0) {                      // 16 codes each; zeros behind the last token
+  const auto fetch = [&](int i0) {                      // 8 codes each; zeros behind the last token
 #pragma unroll
     for (int k = 0; k < kExpandLoads; ++k) {
       const int i = i0 + k * kExpandThreads;
-      const bool in = i >> 3 < live;
-      raw[k] = in ? *reinterpret_cast<const uint4*>(codes + static_cast<size_t>(i) * 16) : make_uint4(0, 0, 0, 0);
-      scale[k] = in ? scales[i >> 3] : 0u;
+      const bool in = i >> 4 < live;
+      raw[k] = in ? *reinterpret_cast<const uint2*>(codes + static_cast<size_t>(i) * 8) : make_uint2(0, 0);
+      scale[k] = in ? scales[i >> 4] : 0u;
     }
   };
   fetch(threadIdx.x);
@@ -262,24 +322,16 @@ __global__ void __launch_bounds__(kExpandThreads) fp8_expand_kernel(
   }
   if (scribe) *entry = to;
   __nv_bfloat16* out = (is_v ? v_out : k_out) + ((static_cast<size_t>(to) * nkv + kvh) * block_size + part * rows) * kFp8D;
-  for (int i0 = threadIdx.x; i0 < rows * 8; i0 += kExpandLoads * kExpandThreads) {
+  for (int i0 = threadIdx.x; i0 < rows * 16; i0 += kExpandLoads * kExpandThreads) {
     if (i0 != threadIdx.x) fetch(i0);
 #pragma unroll
     for (int k = 0; k < kExpandLoads; ++k) {
       const int i = i0 + k * kExpandThreads;
-      if (i >= rows * 8) break;
+      if (i >= rows * 16) break;
       const float m = fp8_scale(scale[k]);
-      const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
-      uint32_t o[8];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 f = fp8_to_float2(w[e]), g = fp8_to_float2(w[e] >> 16);
-        o[2 * e] = pack_bf16x2(f.x * m, f.y * m);
-        o[2 * e + 1] = pack_bf16x2(g.x * m, g.y * m);
-      }
-      uint4* dst = reinterpret_cast<uint4*>(out + static_cast<size_t>(i) * 16);
-      dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
-      dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
+      const float2 f0 = fp8_to_float2(raw[k].x), f1 = fp8_to_float2(raw[k].x >> 16), f2 = fp8_to_float2(raw[k].y), f3 = fp8_to_float2(raw[k].y >> 16);
+      *reinterpret_cast<uint4*>(out + static_cast<size_t>(i) * 8) =
+          make_uint4(pack_bf16x2(f0.x * m, f0.y * m), pack_bf16x2(f1.x * m, f1.y * m), pack_bf16x2(f2.x * m, f2.y * m), pack_bf16x2(f3.x * m, f3.y * m));
     }
   }
 }
@@ -292,7 +344,7 @@ extern "C" int forge_fp8_expand(const void* k_codes, const void* k_scales, const
   if (num_seqs <= 0 || table_width <= 0) return 0;
   if (block_size < 1 || num_seqs > 65535) return -1;
   // a CTA's rows: a page's, or a part of them where there are few pages
-  int rows = std::min(block_size, 32 * kExpandLoads);
+  int rows = std::min(block_size, kExpandLoads * kExpandThreads / 16);
   while (rows > 32 && 2ll * capacity * nkv * (block_size / rows) < 4 * device_sm_count()) rows /= 2;
   const long long z = 2ll * nkv * (block_size / rows);
   if (z > 65535) return -1;
