@@ -8,6 +8,7 @@
 //
 // No counterpart in the reference, whose cache has the model's type.
 #include <algorithm>
+#include <type_traits>
 
 #include "../include/fp8_cache.cuh"
 #include "../include/launch.cuh"
@@ -52,32 +53,43 @@ struct Fp8Store {
   unsigned* status;
 };
 
-// Eight lanes per head, lane j of them has entries 8j.. and 64 + 8j.., the pairs that the rotation mixes; a warp has a set of four heads.  raw: the
-// head's entries; cs: cos and sin of the token at 8j and 64 + 8j, null: no rotation; row0: the slot's row of KV head 0.
-template <bool kVec>
-__device__ __forceinline__ void fp8_store_head(const Fp8Store& a, int t, int h, const uint4* raw, const float* cs, bool slot_ok, size_t row0, int lane) {
+// Eight lanes per head, lane j of them has entries 8j.. and 64 + 8j.., the pairs that the rotation mixes; a warp has a set of four heads.
+enum { kStoreQ = 0, kStoreK = 1, kStoreV = 2 };
+__device__ __forceinline__ int fp8_store_kind(const Fp8Store& a, int h) { return h < a.nq ? kStoreQ : h < a.nq + a.nkv ? kStoreK : kStoreV; }
+
+// A lane's norm weights of query or key heads.
+struct Fp8Weights {
+  float lo[8], hi[8];
+  template <bool kVec>
+  __device__ __forceinline__ void load(const __nv_bfloat16* w, int j) {
+    if (w == nullptr) return;
+    unpack8(load8<kVec>(w + 8 * j), lo);
+    unpack8(load8<kVec>(w + 64 + 8 * j), hi);
+  }
+};
+
+// raw: the head's entries; cs: cos and sin of the token at 8j and 64 + 8j, null: no rotation; row0: the slot's row of KV head 0.
+template <int kKind>
+__device__ __forceinline__ void fp8_store_head(const Fp8Store& a, int t, int h, const uint4* raw, const Fp8Weights& w, const float* cs, bool slot_ok,
+                                               size_t row0, int lane) {
   const int j = lane & 7;
   const unsigned octet = 0xFFu << (lane & 24);           // the lanes of a head; the four heads of a set may be of different kinds
-  const bool is_q = h < a.nq, is_v = h >= a.nq + a.nkv;
   float x[8], y[8], inv = 1.f;
   unpack8(raw[0], x);
   unpack8(raw[1], y);
-  if (!is_v) {
-    const __nv_bfloat16* w = is_q ? a.qw : a.kw;
-    if (w != nullptr) {                                  // the root is a factor of all entries and comes last
-      const uint4 wl = load8<kVec>(w + 8 * j), wh = load8<kVec>(w + 64 + 8 * j);
-      float ss = 0.f, v[8];
+  if constexpr (kKind != kStoreV) {
+    if ((kKind == kStoreQ ? a.qw : a.kw) != nullptr) {   // the root is a factor of all entries and comes last
+      float ss = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], fmaf(y[i], y[i], ss));
 #pragma unroll
       for (int o = 1; o < 8; o <<= 1) ss += __shfl_xor_sync(octet, ss, o);
       inv = rsqrtf(ss * (1.f / kFp8D) + a.eps);
-      unpack8(wl, v);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] *= v[i];
-      unpack8(wh, v);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] *= v[i];
+      for (int i = 0; i < 8; ++i) {
+        x[i] *= w.lo[i];
+        y[i] *= w.hi[i];
+      }
     }
     if (cs != nullptr) {
 #pragma unroll
@@ -90,37 +102,52 @@ __device__ __forceinline__ void fp8_store_head(const Fp8Store& a, int t, int h, 
       }
     }
   }
-  if (is_q) {
+  if constexpr (kKind == kStoreQ) {
     __nv_bfloat16* dst = a.q_out + (static_cast<size_t>(t) * a.nq + h) * kFp8D + 8 * j;
     *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16x2(x[0] * inv, x[1] * inv), pack_bf16x2(x[2] * inv, x[3] * inv), pack_bf16x2(x[4] * inv, x[5] * inv),
                                                 pack_bf16x2(x[6] * inv, x[7] * inv));
     *reinterpret_cast<uint4*>(dst + 64) = make_uint4(pack_bf16x2(y[0] * inv, y[1] * inv), pack_bf16x2(y[2] * inv, y[3] * inv),
                                                      pack_bf16x2(y[4] * inv, y[5] * inv), pack_bf16x2(y[6] * inv, y[7] * inv));
-    return;
-  }
-  float amax = 0.f;
+  } else {
+    float amax = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) amax = max_or_nan(amax, max_or_nan(fabsf(x[i]), fabsf(y[i])));
+    for (int i = 0; i < 8; ++i) amax = max_or_nan(amax, max_or_nan(fabsf(x[i]), fabsf(y[i])));
 #pragma unroll
-  for (int o = 1; o < 8; o <<= 1) amax = max_or_nan(amax, __shfl_xor_sync(octet, amax, o));
-  if (!slot_ok) return;
-  const size_t row = row0 + static_cast<size_t>(is_v ? h - a.nq - a.nkv : h - a.nq) * a.block_size;
-  const uint32_t b = fp8_scale_byte(abs_bits(amax * inv));
-  uint2 code[2] = {make_uint2(kCodesNan, kCodesNan), make_uint2(kCodesNan, kCodesNan)};
-  if (b != kScaleNan) {
-    const float m = fp8_inverse_scale(b);
+    for (int o = 1; o < 8; o <<= 1) amax = max_or_nan(amax, __shfl_xor_sync(octet, amax, o));
+    if (!slot_ok) return;
+    const size_t row = row0 + static_cast<size_t>(kKind == kStoreV ? h - a.nq - a.nkv : h - a.nq) * a.block_size;
+    const uint32_t b = fp8_scale_byte(abs_bits(amax * inv));
+    uint2 code[2] = {make_uint2(kCodesNan, kCodesNan), make_uint2(kCodesNan, kCodesNan)};
+    if (b != kScaleNan) {
+      const float m = fp8_inverse_scale(b);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      x[i] = x[i] * inv * m;
-      y[i] = y[i] * inv * m;
+      for (int i = 0; i < 8; ++i) {
+        x[i] = x[i] * inv * m;
+        y[i] = y[i] * inv * m;
+      }
+      code[0] = make_uint2(fp8_pack(x[0], x[1], x[2], x[3]), fp8_pack(x[4], x[5], x[6], x[7]));
+      code[1] = make_uint2(fp8_pack(y[0], y[1], y[2], y[3]), fp8_pack(y[4], y[5], y[6], y[7]));
     }
-    code[0] = make_uint2(fp8_pack(x[0], x[1], x[2], x[3]), fp8_pack(x[4], x[5], x[6], x[7]));
-    code[1] = make_uint2(fp8_pack(y[0], y[1], y[2], y[3]), fp8_pack(y[4], y[5], y[6], y[7]));
+    uint8_t* dst = (kKind == kStoreV ? a.v_codes : a.k_codes) + row * kFp8D + 8 * j;
+    *reinterpret_cast<uint2*>(dst) = code[0];
+    *reinterpret_cast<uint2*>(dst + 64) = code[1];
+    if (j == 0) (kKind == kStoreV ? a.v_scales : a.k_scales)[row] = static_cast<uint8_t>(b);
   }
-  uint8_t* dst = (is_v ? a.v_codes : a.k_codes) + row * kFp8D + 8 * j;
-  *reinterpret_cast<uint2*>(dst) = code[0];
-  *reinterpret_cast<uint2*>(dst + 64) = code[1];
-  if (j == 0) (is_v ? a.v_scales : a.k_scales)[row] = static_cast<uint8_t>(b);
+}
+// Any head, weights included.
+template <bool kVec>
+__device__ __forceinline__ void fp8_store_any(const Fp8Store& a, int t, int h, const uint4* raw, const float* cs, bool slot_ok, size_t row0, int lane) {
+  Fp8Weights w;
+  const int kind = fp8_store_kind(a, h);
+  if (kind == kStoreQ) {
+    w.load<kVec>(a.qw, lane & 7);
+    fp8_store_head<kStoreQ>(a, t, h, raw, w, cs, slot_ok, row0, lane);
+  } else if (kind == kStoreK) {
+    w.load<kVec>(a.kw, lane & 7);
+    fp8_store_head<kStoreK>(a, t, h, raw, w, cs, slot_ok, row0, lane);
+  } else {
+    fp8_store_head<kStoreV>(a, t, h, raw, w, cs, slot_ok, row0, lane);
+  }
 }
 
 // The slot's row of KV head 0; false: no such slot, or none.
@@ -148,7 +175,7 @@ __global__ void __launch_bounds__(128) fp8_store_kernel(const Fp8Store a) {
   size_t row0;
   const bool slot_ok = fp8_slot_row(a, slot, row0);
   const float* cs = a.rope == nullptr ? nullptr : a.rope + static_cast<size_t>(fp8_angle_row(a, a.positions[t])) * kFp8D + 8 * j;
-  if (h < heads) fp8_store_head<kVec>(a, t, h, raw, cs, slot_ok, row0, lane);
+  if (h < heads) fp8_store_any<kVec>(a, t, h, raw, cs, slot_ok, row0, lane);
 }
 
 // Many tokens: a loading warp brings whole rows of the projection and their angles into a ring by bulk copies, the others take sets of heads
@@ -206,23 +233,45 @@ __global__ void __launch_bounds__(32 * (kStoreWarps + 1), kStoreCtasPerSm) fp8_s
     return;
   }
   const int j = lane & 7;
-  for (int t = blockIdx.x; t < a.T; t += gridDim.x, next()) {
-    if (!mbar_wait(&full[s], phase, a.status)) return;
-    const uint8_t* stage = smem + s * stage_bytes;
-    size_t row0;
-    const bool slot_ok = fp8_slot_row(a, s_slot[s], row0);
-    const float* cs = a.rope == nullptr ? nullptr : reinterpret_cast<const float*>(stage + row_bytes) + 8 * j;
+  const auto walk = [&](auto&& take) {                   // take(token, stage, angles, slot's row, whether there is one)
+    for (int t = blockIdx.x; t < a.T; t += gridDim.x, next()) {
+      if (!mbar_wait(&full[s], phase, a.status)) return;
+      const uint8_t* stage = smem + s * stage_bytes;
+      size_t row0;
+      const bool slot_ok = fp8_slot_row(a, s_slot[s], row0);
+      take(t, stage, a.rope == nullptr ? nullptr : reinterpret_cast<const float*>(stage + row_bytes) + 8 * j, row0, slot_ok);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[s]);
+    }
+  };
+  // one set to a warp, of four heads of one kind: weights and kind are found out once
+  const int h = 4 * warp + (lane >> 3), kind = fp8_store_kind(a, min(h, heads - 1));
+  const auto same = [&](auto k) {
+    Fp8Weights w;
+    if (k.value != kStoreV) w.load<true>(k.value == kStoreQ ? a.qw : a.kw, j);
+    walk([&](int t, const uint8_t* stage, const float* cs, size_t row0, bool slot_ok) {
+      const uint4* src = reinterpret_cast<const uint4*>(stage + h * kFp8D * 2) + j;
+      const uint4 raw[2] = {src[0], src[8]};
+      fp8_store_head<k.value>(a, t, h, raw, w, cs, slot_ok, row0, lane);
+    });
+  };
+  const int first = __shfl_sync(0xffffffffu, kind, 0);   // (by all lanes, whatever their head)
+  if (sets <= consumers && __all_sync(0xffffffffu, h < heads && kind == first)) {
+    if (kind == kStoreQ) same(std::integral_constant<int, kStoreQ>{});
+    else if (kind == kStoreK) same(std::integral_constant<int, kStoreK>{});
+    else same(std::integral_constant<int, kStoreV>{});
+    return;
+  }
+  walk([&](int t, const uint8_t* stage, const float* cs, size_t row0, bool slot_ok) {
     for (int set = warp; set < sets; set += consumers) {
-      const int h = 4 * set + (lane >> 3);
-      if (h < heads) {
-        const uint4* src = reinterpret_cast<const uint4*>(stage + h * kFp8D * 2) + j;
+      const int head = 4 * set + (lane >> 3);
+      if (head < heads) {
+        const uint4* src = reinterpret_cast<const uint4*>(stage + head * kFp8D * 2) + j;
         const uint4 raw[2] = {src[0], src[8]};
-        fp8_store_head<true>(a, t, h, raw, cs, slot_ok, row0, lane);
+        fp8_store_any<true>(a, t, head, raw, cs, slot_ok, row0, lane);
       }
     }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&empty[s]);
-  }
+  });
 }
 
 // qkv [T, (nq + 2 nkv) * 128] with rows ld apart; rope fp32 [rope_rows][128] = cos, sin; slot < 0 is passed over, slot >= num_slots too and
