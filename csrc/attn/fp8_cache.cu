@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(128) fp8_store_kernel(const Fp8Store a) {
 // Many tokens: a loading warp brings whole rows of the projection and their angles into a ring by bulk copies, the others take sets of heads
 // from it, so that memory is asked ahead of the arithmetic whatever that takes.  Persistent, two CTAs per SM; shared memory is asked for
 // so that no third fits beside them: of equal shares none may wait for a CTA that another SM would have had room for.
-constexpr int kStoreRing = 1024;                       // tokens from which on
+constexpr int kStoreRingTokens = 2048, kStoreRingSets = 8;         // from which on
 constexpr int kStoreWarps = 12, kStoreCtasPerSm = 2, kStoreSmem = 108 * 1024, kStoreMaxStages = 8;
 
 __global__ void __launch_bounds__(32 * (kStoreWarps + 1), kStoreCtasPerSm) fp8_store_ring_kernel(const Fp8Store a, int stages) {
@@ -292,7 +292,10 @@ extern "C" int forge_fp8_store(const void* qkv, long long ld, const void* qw, co
   const bool vec = ld % 8 == 0 && aligned(qkv) && aligned(qw) && aligned(kw);
   const int heads = nq + 2 * nkv, sets = (heads + 3) / 4, stage = heads * kFp8D * 2 + kFp8D * 4;
   const int stages = std::min(kStoreMaxStages, kStoreSmem / stage);
-  if (vec && stages >= 3 && T >= kStoreRing) {
+  // Measured, a warp per set / ring, us: 32 + 16 heads, 1024 tokens 6.2 / 6.1, 2048: 12.8 / 10.5, 4001: 23.8 / 18.7, 8192: 45 / 35; 16 + 16 heads, 1024:
+  // 4.8 / 5.1, 2048: 7.8 / 8.1, 4001: 16.4 / 15.0; 64 + 16 heads (two sets to a warp), 1024: 9.7 / 11.3, 2048: 20.2 / 20.9, 4001: 39 / 36; 8 + 2 heads
+  // (three warps at work), 4001: 6.8 / 16.1.
+  if (vec && stages >= 3 && T >= kStoreRingTokens && sets >= kStoreRingSets) {
     FORGE_ENSURE_DYN_SMEM(fp8_store_ring_kernel, kStoreSmem);
     const int ctas = std::min(T, kStoreCtasPerSm * device_sm_count());
     return launch_kernel(fp8_store_ring_kernel, dim3(ctas), dim3(32 * (std::min(sets, kStoreWarps) + 1)), kStoreSmem, stream, 0, a, stages) == cudaSuccess
