@@ -3,7 +3,7 @@
 output tokens/s (device time of the engine steps, max over ranks; and end to end), and the mean decode step time.
 
     python bench_decode.py [--model qwen3-32b] [--gpus N] [--requests 64] [--prompt 2048] [--out 512]
-                           [--quantization fp8_block] [--impl ours|reference]
+                           [--quantization fp8_block] [--kv-cache fp8] [--impl ours|reference]
 
 With --gpus N > 1 launch under torchrun (one rank per GPU), like bench.py.  ``--impl reference`` runs the reference
 engine from ``baseline/_ref`` on the same requests (bf16 only; its weights are initialised on the device instead of
@@ -43,6 +43,8 @@ def run_ours(args, max_len):
               max_num_seqs=max(args.requests, 16), comm=args.comm, extra={"device_timing": True})
     if args.quantization != "none":
         kw["quantization"] = args.quantization
+    if args.kv_cache != "none":
+        kw["kv_cache_dtype"] = args.kv_cache
     llm = LLM(args.model, hf_config=preset(args.model), load_format="dummy", skip_tokenizer_init=True, **kw)
     sp = SamplingParams(temperature=0.6, max_tokens=args.out, ignore_eos=True)
     for p in range(args.warmup):
@@ -72,7 +74,7 @@ def run_reference(args, max_len):
     n = args.gpus
     if n > 1 and int(os.environ.get("RANK", "0")) != 0:
         return None
-    if args.quantization != "none":
+    if args.quantization != "none" or args.kv_cache != "none":
         return {"impl": "reference", "unavailable": "the reference has no fp8 path"}
     import torch
     from tinyllmforge_b200 import preset
@@ -120,6 +122,7 @@ def main():
     ap.add_argument("--warmup", type=int, default=1)
     ap.add_argument("--comm", default="fused", choices=["fused", "nccl"])
     ap.add_argument("--quantization", default="none", choices=["none", "fp8_block"])
+    ap.add_argument("--kv-cache", default="none", choices=["none", "fp8"])
     ap.add_argument("--impl", default="ours", choices=["ours", "reference"])
     args = ap.parse_args()
     max_len = args.prompt + args.out + 64

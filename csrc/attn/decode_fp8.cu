@@ -497,7 +497,7 @@ constexpr int kF8JoinWarps = 8;
 
 __global__ void __launch_bounds__(32 * kF8JoinWarps) decode_fp8_join_kernel(const Fp8Decode a) {
   __shared__ float4 s_o[kF8JoinWarps][32];
-  __shared__ float s_l[kF8JoinWarps];
+  __shared__ float2 s_ml[kF8JoinWarps];
   pdl_launch_dependents();
   pdl_wait();
   const int me = blockIdx.x, head = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -505,31 +505,35 @@ __global__ void __launch_bounds__(32 * kF8JoinWarps) decode_fp8_join_kernel(cons
   const int parts = cut.x, kvh = cut.z / a.slices, slice = cut.z - kvh * a.slices;
   if (parts == 0 || head >= min(a.G, a.group - slice * a.G)) return;
   const auto slot = [&](int i) { return static_cast<size_t>(i == 0 ? 2 * (me - 1) + 1 : 2 * (me + i - 1)) * a.G + head; };
-  float M = -INFINITY, L = 0.f;
+  float M = -INFINITY, L = 0.f;                          // of the warp's parts
   float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i = lane; i < parts; i += 32) M = fmaxf(M, a.part_ml[2 * slot(i)]);
-#pragma unroll
-  for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
 #pragma unroll 4
   for (int i = warp; i < parts; i += kF8JoinWarps) {
     const size_t p = slot(i);
     const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * p);
     const float4 v = *reinterpret_cast<const float4*>(a.part_o + p * kFp8D + 4 * lane);
-    const float f = (ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - M)) * ml.y;
-    L += f;
-    O.x = fmaf(f, v.x, O.x);
-    O.y = fmaf(f, v.y, O.y);
-    O.z = fmaf(f, v.z, O.z);
-    O.w = fmaf(f, v.w, O.w);
+    const float m = fmaxf(M, ml.x);
+    const float keep = M == -INFINITY ? 0.f : ex2_approx(M - m), f = (ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - m)) * ml.y;
+    M = m;
+    L = L * keep + f;
+    O.x = O.x * keep + f * v.x;
+    O.y = O.y * keep + f * v.y;
+    O.z = O.z * keep + f * v.z;
+    O.w = O.w * keep + f * v.w;
   }
   s_o[warp][lane] = O;
-  if (lane == 0) s_l[warp] = L;
+  if (lane == 0) s_ml[warp] = make_float2(M, L);
   __syncthreads();
   if (warp != 0) return;
-  for (int i = 1; i < min(kF8JoinWarps, parts); ++i) {
+  const int n = min(kF8JoinWarps, parts);
+  for (int i = 0; i < n; ++i) M = fmaxf(M, s_ml[i].x);
+  L = 0.f;
+  O = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; i < n; ++i) {
     const float4 v = s_o[i][lane];
-    O.x += v.x; O.y += v.y; O.z += v.z; O.w += v.w;
-    L += s_l[i];
+    const float f = s_ml[i].x == -INFINITY ? 0.f : ex2_approx(s_ml[i].x - M);
+    L += f * s_ml[i].y;
+    O.x += f * v.x; O.y += f * v.y; O.z += f * v.z; O.w += f * v.w;
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;
   const int h = kvh * a.group + slice * a.G + head;

@@ -8,6 +8,7 @@ import torch
 from tinyllmforge_b200 import LLM, Config, SamplingParams, preset
 from tinyllmforge_b200.ops import ref
 from tinyllmforge_b200.ops.quant import Fp8BlockWeight, Fp8KVCache, Fp8Rows, linear_fp8_ref, quantize_heads
+from tinyllmforge_b200.utils.synth import write_checkpoint
 
 F64 = torch.float64
 
@@ -152,6 +153,22 @@ def test_engine_serves_from_an_8_bit_cache(quantization):
     assert sum(a == b for s, t in zip(whole, chunked) for a, b in zip(s, t)) >= 0.9 * 32
     plain, cache, _ = _tokens(prompts, kv_cache_dtype=None, quantization=quantization)
     assert isinstance(cache, torch.Tensor) and len(plain) == 4
+
+
+def test_two_ranks_serve_from_8_bit_caches_of_their_heads(tmp_path):
+    path = str(tmp_path / "tiny")
+    write_checkpoint(path, preset("tiny"), seed=0, std=0.2, norm_std=0.1)
+    rng = random.Random(1)
+    prompts = [[rng.randrange(4096) for _ in range(n)] for n in (5, 40, 100)]
+    tokens = []
+    for size in (1, 2):
+        llm = LLM(path, device="cpu", kvcache_block_size=16, max_model_len=256, max_num_batched_tokens=256, num_kvcache_blocks=64, kv_cache_dtype="fp8",
+                  tensor_parallel_size=size)
+        tokens.append([o["token_ids"] for o in llm.generate(prompts, SamplingParams(temperature=0.0, max_tokens=8, ignore_eos=True), use_tqdm=False)])
+        assert llm.worker.model.kv_cache.shape[3] == 2 // size         # KV heads of a rank
+        llm.exit()
+    # the ranks' sums are added in another order: 2^-24 of an entry, which moves few codes over a border
+    assert sum(a == b for s, t in zip(*tokens) for a, b in zip(s, t)) >= 0.9 * 24
 
 
 def test_block_bytes_and_norms_in_8_bits_follow_the_options():

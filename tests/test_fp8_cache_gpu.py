@@ -345,6 +345,32 @@ def test_calls_without_tokens(ops):
     assert ops.expand_kv(kc, vc, none.block_tables, none.context_lens, 0)[0].shape == (0, 2, 16, 128)
 
 
+@pytest.mark.parametrize("mode", ["flat", "chunked"])
+def test_blocks_beyond_four_gigabytes(ops, mode, monkeypatch):
+    """Codes whose byte offsets do not fit 32 bits: stored, attended to and read back at the end of a large cache."""
+    monkeypatch.setattr(ops, "decode_attention_mode", mode)
+    blocks, bs, nq, nkv, n = 140_000, 256, 4, 1, 300
+    assert blocks * bs * 128 > 2 ** 32
+    caches = [Fp8KVCache.zeros(blocks, nkv, bs, 128, device="cuda") for _ in range(2)]
+    gen = _gen(7)
+    order = _ints([blocks - 1, blocks - 2])
+    qkv = _randn(gen, n, (nq + 2 * nkv) * 128).to(BF)
+    pos = torch.arange(n, device="cuda")
+    slots = order[0, pos // bs].long() * bs + pos % bs
+    assert int(slots.max()) < 2 ** 31
+    q = ops.qk_norm_rope_store(qkv, None, None, 1e-6, ref.rope_table(512, 128, 1e6, "cuda"), pos.int(), slots.int(), *caches, nq, nkv, 128, do_rope=False)
+    heads = qkv.view(n, 6, 128)
+    for c, x in zip(caches, (heads[:, 4], heads[:, 5])):
+        codes, _ = quantize_heads(x.float())
+        assert torch.equal(c.code_bytes[order[0].long()].reshape(512, 128)[:n], codes.view(torch.uint8))
+    step = Step(is_prefill=False, num_seqs=1, padded_seqs=1, table_width=2, max_seqlen_k=n, block_tables=order, context_lens=_ints(n))
+    _check_decode(ops.attention(q[-1:].contiguous(), *caches, step, SCALE), q[-1:], *caches, step, [n])
+    k, v, _ = ops.expand_kv(*caches, order, step.context_lens, 2)
+    for got, c in ((k, caches[0]), (v, caches[1])):
+        assert torch.equal(got.reshape(512, 128)[:n].float(), c[order[0].long()].dequantize().reshape(512, 128)[:n])
+    ops.check_status()
+
+
 # ----------------------------------------------------------------------------- norm
 @pytest.mark.parametrize("M,H", [(1, 128), (1, 4096), (5, 384), (61, 5120), (3, 16384), (2050, 2560), (130, 1152)])
 @pytest.mark.parametrize("residual", [False, True])
