@@ -52,9 +52,10 @@ class Fp8Ops:
                 pages += -(-lens[end] // bs)
                 end += 1
             part = slice(begin, end)
-            k, v, tables = self.expand_kv(k_cache, v_cache, batch.block_tables[part], batch.context_lens[part], pages)
-            self.C.prefill_attention(q, k, v, batch.cu_seqlens_q[begin:end + 1], batch.context_lens[part], tables, out, end - begin,
-                                     batch.max_seqlen_q, scale, self.status)
+            if pages:                             # (sequences without keys have no queries either)
+                k, v, tables = self.expand_kv(k_cache, v_cache, batch.block_tables[part], batch.context_lens[part], pages)
+                self.C.prefill_attention(q, k, v, batch.cu_seqlens_q[begin:end + 1], batch.context_lens[part], tables, out, end - begin,
+                                         batch.max_seqlen_q, scale, self.status)
             begin = end
         return out
 
