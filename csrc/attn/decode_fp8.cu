@@ -21,7 +21,8 @@
 // The split, many items.  The tiles of 64 tokens of all items, in order, are dealt out to four teams per SM, of two consumer warps and a loading one with a
 // ring each: an item counts as its tiles and kF8ItemCost more for its beginning and end, and team i of C takes the i-th of C equal shares,
 // so short and long contexts, few and many sequences fill the GPU alike.  An item inside one team is finished there; the parts of one that
-// is cut are joined by a second kernel.  Lengths are read on the device, so the launch fits a CUDA graph whatever they become.
+// is cut are joined by a second kernel, in order, so that the same step gives the same bits; how an item is cut depends on the others, and
+// with it the last bits of its sums.  Lengths are read on the device, so the launch fits a CUDA graph whatever they become.
 // The four teams of an SM are one CTA: as CTAs of their own, launched beside the end of another kernel (PDL), some SMs took only
 // three, and the others ran after all the rest (256 sequences of 100 .. 1500 tokens: 82 us after an idle GPU, 116 in a row).
 // The split, few items of moderate length.  A cluster of one to eight CTAs takes an item, each a run of its tiles of 128 tokens, and they join what they
@@ -331,8 +332,8 @@ struct F8State {
 // ---------------------------------------------------------------------------------------------------------
 constexpr int kF8Warps = 2, kF8Stages = 3, kF8Teams = 4;
 constexpr int kF8TeamWarps = kF8Warps + 1, kF8Threads = 32 * kF8Teams * kF8TeamWarps;
-constexpr int kF8ItemCost = 2;                         // tiles
-constexpr int kF8Share = 4;                            // no team gets less than this
+constexpr int kF8ItemCost = 2;                         // tiles (1, 3: 256 x 100 .. 1500 81.8, 76.3 us for 75.7)
+constexpr int kF8Share = 4;                            // units to a team at least, or there are fewer teams at work (2, 8: 13 x 200 .. 2000 13.7, 16.7 us for 13.4)
 using F8FlatRing = F8Ring<kF8Warps, kF8Stages>;
 
 constexpr int kF8JoinArea = (kF8Warps - 1) * F8State::kJoinFloats;

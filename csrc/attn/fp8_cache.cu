@@ -74,21 +74,21 @@ __device__ __forceinline__ void fp8_store_head(const Fp8Store& a, int t, int h, 
                                                size_t row0, int lane) {
   const int j = lane & 7;
   const unsigned octet = 0xFFu << (lane & 24);           // the lanes of a head; the four heads of a set may be of different kinds
-  float x[8], y[8], inv = 1.f;
+  float x[8], y[8];
   unpack8(raw[0], x);
   unpack8(raw[1], y);
   if constexpr (kKind != kStoreV) {
-    if ((kKind == kStoreQ ? a.qw : a.kw) != nullptr) {   // the root is a factor of all entries and comes last
+    if ((kKind == kStoreQ ? a.qw : a.kw) != nullptr) {
       float ss = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], fmaf(y[i], y[i], ss));
 #pragma unroll
       for (int o = 1; o < 8; o <<= 1) ss += __shfl_xor_sync(octet, ss, o);
-      inv = rsqrtf(ss * (1.f / kFp8D) + a.eps);
+      const float inv = rsqrtf(ss * (1.f / kFp8D) + a.eps);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        x[i] *= w.lo[i];
-        y[i] *= w.hi[i];
+        x[i] = x[i] * inv * w.lo[i];
+        y[i] = y[i] * inv * w.hi[i];
       }
     }
     if (cs != nullptr) {
@@ -104,10 +104,8 @@ __device__ __forceinline__ void fp8_store_head(const Fp8Store& a, int t, int h, 
   }
   if constexpr (kKind == kStoreQ) {
     __nv_bfloat16* dst = a.q_out + (static_cast<size_t>(t) * a.nq + h) * kFp8D + 8 * j;
-    *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16x2(x[0] * inv, x[1] * inv), pack_bf16x2(x[2] * inv, x[3] * inv), pack_bf16x2(x[4] * inv, x[5] * inv),
-                                                pack_bf16x2(x[6] * inv, x[7] * inv));
-    *reinterpret_cast<uint4*>(dst + 64) = make_uint4(pack_bf16x2(y[0] * inv, y[1] * inv), pack_bf16x2(y[2] * inv, y[3] * inv),
-                                                     pack_bf16x2(y[4] * inv, y[5] * inv), pack_bf16x2(y[6] * inv, y[7] * inv));
+    *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+    *reinterpret_cast<uint4*>(dst + 64) = make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7]));
   } else {
     float amax = 0.f;
 #pragma unroll
@@ -116,17 +114,12 @@ __device__ __forceinline__ void fp8_store_head(const Fp8Store& a, int t, int h, 
     for (int o = 1; o < 8; o <<= 1) amax = max_or_nan(amax, __shfl_xor_sync(octet, amax, o));
     if (!slot_ok) return;
     const size_t row = row0 + static_cast<size_t>(kKind == kStoreV ? h - a.nq - a.nkv : h - a.nq) * a.block_size;
-    const uint32_t b = fp8_scale_byte(abs_bits(amax * inv));
+    const uint32_t b = fp8_scale_byte(abs_bits(amax));
     uint2 code[2] = {make_uint2(kCodesNan, kCodesNan), make_uint2(kCodesNan, kCodesNan)};
     if (b != kScaleNan) {
       const float m = fp8_inverse_scale(b);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[i] = x[i] * inv * m;
-        y[i] = y[i] * inv * m;
-      }
-      code[0] = make_uint2(fp8_pack(x[0], x[1], x[2], x[3]), fp8_pack(x[4], x[5], x[6], x[7]));
-      code[1] = make_uint2(fp8_pack(y[0], y[1], y[2], y[3]), fp8_pack(y[4], y[5], y[6], y[7]));
+      code[0] = make_uint2(fp8_pack(x[0] * m, x[1] * m, x[2] * m, x[3] * m), fp8_pack(x[4] * m, x[5] * m, x[6] * m, x[7] * m));
+      code[1] = make_uint2(fp8_pack(y[0] * m, y[1] * m, y[2] * m, y[3] * m), fp8_pack(y[4] * m, y[5] * m, y[6] * m, y[7] * m));
     }
     uint8_t* dst = (kKind == kStoreV ? a.v_codes : a.k_codes) + row * kFp8D + 8 * j;
     *reinterpret_cast<uint2*>(dst) = code[0];

@@ -346,6 +346,18 @@ def test_calls_without_tokens(ops):
 
 
 @pytest.mark.parametrize("mode", ["flat", "chunked"])
+def test_decode_over_a_long_context_with_a_common_direction(ops, mode, monkeypatch):
+    """200000 values of one sign: sums that lose a little at every step would be off by the same sign."""
+    monkeypatch.setattr(ops, "decode_attention_mode", mode)
+    lens = [200_000]
+    q, kc, vc, step = _paged(lens, 4, 1, 256, q_scale=0.5)
+    v = quantize_heads(1.0 + 0.2 * _randn(_gen(4), *vc.shape))
+    live = vc.scales != 255
+    vc.code_bytes[live], vc.scales[live] = v[0].view(torch.uint8)[live], v[1][live]
+    _check_decode(ops.attention(q, kc, vc, step, SCALE), q, kc, vc, step, lens)
+
+
+@pytest.mark.parametrize("mode", ["flat", "chunked"])
 def test_blocks_beyond_four_gigabytes(ops, mode, monkeypatch):
     """Codes whose byte offsets do not fit 32 bits: stored, attended to and read back at the end of a large cache."""
     monkeypatch.setattr(ops, "decode_attention_mode", mode)

@@ -35,7 +35,7 @@ class Fp8Ops:
     def decode_attention_fp8(self, q, k_cache, v_cache, batch, scale):
         """``decode_attention_mode``: "flat" equal shares over the GPU, "chunked" a cluster of CTAs per sequence and KV head, "auto" by size."""
         return self.C.decode_fp8(q, *self._halves(k_cache, v_cache), batch.block_tables, batch.context_lens, scale, self.status,
-                                 _DECODE_MODES[self.decode_attention_mode])
+                                 _DECODE_MODES.get(self.decode_attention_mode, 2))
 
     def prefill_attention_fp8(self, q, k_cache, v_cache, batch, scale):
         """Prompts: the sequences' pages are read back and attended to by the bf16 kernels, as many sequences at a time as have
