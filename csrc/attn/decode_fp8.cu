@@ -149,8 +149,13 @@ struct F8State {
     for (int i = 0; i < 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
   }
 
-  // 32 tokens; of them `valid` (1 or more) count.  K, V: their rows, of a 1024-byte aligned tile with the 128-byte swizzle.
+  // 32 tokens; of them `valid` (1 or more; kWhole: all) count.  K, V: their rows, of a 1024-byte aligned tile with the 128-byte swizzle.
   __device__ __forceinline__ void take(const uint8_t* K, const uint8_t* V, const uint8_t* k_scales, const uint8_t* v_scales, int valid, int lane) {
+    if (valid >= 32) take_tokens<true>(K, V, k_scales, v_scales, 32, lane);
+    else take_tokens<false>(K, V, k_scales, v_scales, valid, lane);
+  }
+  template <bool kWhole>
+  __device__ __forceinline__ void take_tokens(const uint8_t* K, const uint8_t* V, const uint8_t* k_scales, const uint8_t* v_scales, int valid, int lane) {
     const int g = lane >> 2, quad = lane & 3;
     // ---- products
     float c[2][2][4];
@@ -186,7 +191,7 @@ struct F8State {
         y[i][h] = x[i][h] + e;
       }
     }
-    if (valid < 32) {
+    if constexpr (!kWhole) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         if (8 * i + g >= valid) x[i][0] = x[i][1] = y[i][0] = y[i][1] = -INFINITY;
@@ -218,15 +223,14 @@ struct F8State {
         }
       }
     }
-    // ---- weights; without a finite score so far (NaN) any reference does
+    // ---- weights.  A token that counts has given each maximum a value, or its score is not finite and the result is NaN.
     uint32_t p[4];
     {
-      const float m0 = m[0] == -INFINITY ? 0.f : m[0], m1 = m[1] == -INFINITY ? 0.f : m[1];
-      const float u0 = (u[0] == -INFINITY ? 0.f : u[0]) - kF8Top, u1 = (u[1] == -INFINITY ? 0.f : u[1]) - kF8Top;
+      const float u0 = u[0] - kF8Top, u1 = u[1] - kF8Top;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        l[0] += ex2_approx(x[i][0] - m0);                // -inf -> 0
-        l[1] += ex2_approx(x[i][1] - m1);
+        l[0] += ex2_approx(x[i][0] - m[0]);              // -inf -> 0
+        l[1] += ex2_approx(x[i][1] - m[1]);
         p[i] = transpose8x8(f8_half2(ex2_approx(y[i][0] - u0), ex2_approx(y[i][1] - u1)));
       }
     }
@@ -238,7 +242,7 @@ struct F8State {
       for (int h = 0; h < 4; ++h) {
         const int tok = 16 * t + 2 * quad + (h & 1) + 8 * (h >> 1);
         uint4 v = *reinterpret_cast<const uint4*>(V + tok * kFp8D + ((g ^ (tok & 7)) << 4));
-        if (valid < 32 && tok >= valid) v = make_uint4(0, 0, 0, 0);
+        if (!kWhole && tok >= valid) v = make_uint4(0, 0, 0, 0);
         w[h][0] = v.x; w[h][1] = v.y; w[h][2] = v.z; w[h][3] = v.w;
       }
 #pragma unroll
@@ -454,7 +458,7 @@ decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       st.begin(a.q + (static_cast<size_t>(seq) * a.nq + head0) * kFp8D, heads, a.scale_log2, lane);
       for (int i = 0; i < count; ++i, ring.next()) {
         const int valid = len - (j + i) * F8FlatRing::kTile - 32 * warp;
-        ok = ok && mbar_wait(&ring.full[ring.s], ring.phase, a.status);
+        ok = ok && mbar_wait_parked(&ring.full[ring.s], ring.phase, a.status);
         if (valid > 0) {
           const uint8_t* K = ring.codes + ring.s * 2 * F8FlatRing::kHalf + 32 * warp * kFp8D;
           const uint8_t* sc = ring.scales + ring.s * 2 * F8FlatRing::kTile + 32 * warp;
@@ -597,7 +601,7 @@ decode_fp8_cluster_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid
     bool ok = true;
     for (int i = 0; i < count; ++i, ring.next()) {
       const int valid = len - (j + i) * F8ClusterRing::kTile - 32 * warp;
-      ok = ok && mbar_wait(&ring.full[ring.s], ring.phase, a.status);
+      ok = ok && mbar_wait_parked(&ring.full[ring.s], ring.phase, a.status);
       if (valid > 0) {
         const uint8_t* K = ring.codes + ring.s * 2 * F8ClusterRing::kHalf + 32 * warp * kFp8D;
         const uint8_t* sc = ring.scales + ring.s * 2 * F8ClusterRing::kTile + 32 * warp;
