@@ -1,6 +1,7 @@
 // Bindings of the ops that keep keys, values and normed rows in 8 bits.  As in bindings.cpp every argument is checked here (device, type,
 // contiguity, shapes, alignment), so a malformed call raises in Python instead of reaching a kernel.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -30,6 +31,10 @@ constexpr auto BF = at::kBFloat16;
 constexpr auto U8 = at::kByte;
 constexpr auto E4M3 = at::kFloat8_e4m3fn;
 
+// An uninitialised tensor beside `like`, without the way through the dispatcher: half a microsecond each, of calls of eight.
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt);
+}
 void same_device(const Tensor& a, const Tensor& b, const char* what) { TORCH_CHECK(a.device() == b.device(), what, ": tensors on one device expected"); }
 void aligned16(const Tensor& t, const char* what) { TORCH_CHECK((reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0, what, ": 16-byte alignment needed"); }
 
@@ -83,7 +88,7 @@ Tensor fp8_store(const Tensor& qkv, const OptTensor& qw, const OptTensor& kw, do
   same_device(slots, qkv, "fp8_store");
   same_device(status, qkv, "fp8_store");
   const c10::cuda::CUDAGuard guard(qkv.device());
-  Tensor q = at::empty({T, nq, 128}, qkv.options());
+  Tensor q = fresh({T, nq, 128}, BF, qkv);
   check_rc(forge_fp8_store(qkv.data_ptr(), T > 1 ? qkv.stride(0) : qkv.size(1), norm_weight(qw, qkv, "fp8_store"), norm_weight(kw, qkv, "fp8_store"),
                            static_cast<float>(eps), rp, rope_rows, ints(positions, T, "fp8_store: positions"), ints(slots, T, "fp8_store: slots"), q.data_ptr(),
                            k.codes, k.scales, v.codes, v.scales, i32(T), i32(nq), i32(k.nkv), i32(k.block), k.blocks * k.block,
@@ -104,9 +109,8 @@ std::tuple<Tensor, Tensor, Tensor> fp8_expand(const Tensor& k_codes, const Tenso
   const int* bt = ints(block_tables, S * W, "fp8_expand: tables");
   const int* ln = ints(lens, S, "fp8_expand: lengths");
   const c10::cuda::CUDAGuard guard(k_codes.device());
-  const auto bf16 = k_codes.options().dtype(BF);
-  Tensor k_out = at::empty({pages, k.nkv, k.block, 128}, bf16), v_out = at::empty({pages, k.nkv, k.block, 128}, bf16);
-  Tensor tables = at::empty({S, W}, block_tables.options());
+  Tensor k_out = fresh({pages, k.nkv, k.block, 128}, BF, k_codes), v_out = fresh({pages, k.nkv, k.block, 128}, BF, k_codes);
+  Tensor tables = fresh({S, W}, at::kInt, k_codes);
   check_rc(forge_fp8_expand(k.codes, k.scales, v.codes, v.scales, bt, ln, i32(S), i32(W), i32(k.blocks), i32(k.nkv), i32(k.block), k_out.data_ptr(),
                             v_out.data_ptr(), tables.data_ptr<int>(), i32(pages), status_word(status), stream_of(k_codes)),
            "forge_fp8_expand");
@@ -129,10 +133,10 @@ Tensor decode_fp8(const Tensor& q, const Tensor& k_codes, const Tensor& k_scales
   const int* bt = ints(block_tables, B * W, "decode_fp8: tables");
   const int* ln = ints(lens, B, "decode_fp8: lengths");
   const c10::cuda::CUDAGuard guard(q.device());
-  Tensor out = at::empty({B, nq * 128}, q.options());
+  Tensor out = fresh({B, nq * 128}, BF, q);
   const int64_t floats = forge_decode_fp8_scratch_floats(i32(B), i32(nq), i32(k.nkv), i32(k.block), i32(W), i32(mode));
   Tensor scratch;
-  if (floats > 0) scratch = at::empty({floats}, q.options().dtype(at::kFloat));
+  if (floats > 0) scratch = fresh({floats}, at::kFloat, q);
   check_rc(forge_decode_fp8(qp, k.codes, k.scales, v.codes, v.scales, bt, ln, out.data_ptr(), floats > 0 ? scratch.data_ptr<float>() : nullptr, i32(B), i32(nq),
                             i32(k.nkv), i32(k.block), i32(W), i32(k.blocks), static_cast<float>(scale), i32(mode), status_word(status), stream_of(q)),
            "forge_decode_fp8");
@@ -157,7 +161,7 @@ std::tuple<Tensor, Tensor> rms_norm_fp8(const Tensor& x, const OptTensor& residu
   if (M > 0) aligned16(x, "rms_norm_fp8: x");
   aligned16(w, "rms_norm_fp8: weight");
   const c10::cuda::CUDAGuard guard(x.device());
-  Tensor codes = at::empty({M, H}, x.options().dtype(E4M3)), scales = at::empty({H / 128, (M + 3) / 4 * 4}, x.options().dtype(at::kFloat));
+  Tensor codes = fresh({M, H}, E4M3, x), scales = fresh({H / 128, (M + 3) / 4 * 4}, at::kFloat, x);
   check_rc(forge_rms_norm_fp8(xp, res, wp, codes.data_ptr(), scales.data_ptr<float>(), i32(scales.size(1)), i32(M), i32(H), static_cast<float>(eps),
                               stream_of(x)),
            "forge_rms_norm_fp8");
