@@ -88,18 +88,27 @@ struct F8Ring {
       mbar_init(&empty[i], kWarps);
     }
   }
-  // One thread: tiles [j, j + count) of a sequence with `len` tokens.  False: a wait has run out.
-  __device__ __forceinline__ bool load(const Fp8Decode& a, const CUtensorMap* tm_k, const CUtensorMap* tm_v, int seq, int kvh, int len, int j, int count) {
+  // A warp: tiles [j, j + count) of a sequence with `len` tokens.  `held`: the lane's of 32 table entries from page `from` on.  False: a wait has
+  // run out.
+  __device__ __forceinline__ bool load(const Fp8Decode& a, const CUtensorMap* tm_k, const CUtensorMap* tm_v, int seq, int kvh, int len, int j, int count,
+                                       int from, int held, int lane) {
     const int rows = min(a.block_size, kTile);
-    const int* table = a.block_tables + static_cast<size_t>(seq) * a.table_width;
     for (const int end = j + count; j < end; ++j) {
       const int tok0 = j * kTile, pages = (min(len - tok0, kTile) + rows - 1) / rows;
-      int blk = table[tok0 / a.block_size];              // asked for before the wait
-      if (!mbar_wait_parked(&empty[s], phase ^ 1, a.status)) return false;
-      mbar_expect_tx(&full[s], pages * rows * 2 * (kFp8D + 1));
+      bool ok = true;
+      if (lane == 0) {
+        ok = mbar_wait_parked(&empty[s], phase ^ 1, a.status);
+        if (ok) mbar_expect_tx(&full[s], pages * rows * 2 * (kFp8D + 1));
+      }
+      if (!__shfl_sync(0xffffffffu, ok, 0)) return false;
       for (int p = 0; p < pages; ++p) {
-        const int tok = tok0 + p * rows;
-        if (p > 0) blk = table[tok / a.block_size];
+        const int tok = tok0 + p * rows, page = tok / a.block_size;
+        if (page >= from + 32) {
+          from = page;
+          held = entry(a, seq, page + lane);
+        }
+        int blk = __shfl_sync(0xffffffffu, held, page - from);
+        if (lane != 0) continue;
         if (blk < 0 || blk >= a.num_blocks) {
           set_status(a.status, kStatusBadIndex);
           blk = 0;
@@ -112,9 +121,13 @@ struct F8Ring {
         bulk_load(sc, a.k_scales + row, rows, &full[s]);
         bulk_load(sc + kTile, a.v_scales + row, rows, &full[s]);
       }
+      __syncwarp();
       next();
     }
     return true;
+  }
+  static __device__ __forceinline__ int entry(const Fp8Decode& a, int seq, int page) {
+    return page < a.table_width ? a.block_tables[static_cast<size_t>(seq) * a.table_width + page] : -1;
   }
 };
 
@@ -453,7 +466,8 @@ decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     const int count = min(n - j, u_end - (base + kF8ItemCost + j)), len = min(a.lens[seq], cap);
     const int kvh = item / a.slices, slice = item - kvh * a.slices, head0 = kvh * a.group + slice * a.G, heads = min(a.G, a.group - slice * a.G);
     if (warp == kF8Warps) {
-      if (lane == 0 && ok) ok = ring.load(a, &tm_k, &tm_v, seq, kvh, len, j, count);
+      const int from = j * F8FlatRing::kTile / a.block_size;
+      if (ok) ok = ring.load(a, &tm_k, &tm_v, seq, kvh, len, j, count, from, ring.entry(a, seq, from + lane), lane);
     } else {
       st.begin(a.q + (static_cast<size_t>(seq) * a.nq + head0) * kFp8D, heads, a.scale_log2, lane);
       for (int i = 0; i < count; ++i, ring.next()) {
@@ -551,7 +565,7 @@ __global__ void __launch_bounds__(32 * kF8JoinWarps, 8) decode_fp8_join_kernel(c
 // ---------------------------------------------------------------------------------------------------------
 // Few items: a cluster of CTAs each
 // ---------------------------------------------------------------------------------------------------------
-constexpr int kF8CWarps = 4, kF8CStages = 2, kF8CThreads = 32 * (kF8CWarps + 1), kF8CCtasPerSm = 3;
+constexpr int kF8CWarps = 4, kF8CStages = 2, kF8CThreads = 32 * (kF8CWarps + 1), kF8CCtasPerSm = 2;
 using F8ClusterRing = F8Ring<kF8CWarps, kF8CStages>;
 constexpr int f8_cluster_smem(int G) {
   return 1024 + F8ClusterRing::kBytes + (kF8CWarps - 1) * F8State::kJoinFloats * 4 + G * (kFp8D + 2) * 4 + 2 * kF8CStages * 8;
@@ -586,6 +600,7 @@ decode_fp8_cluster_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid
   const int kvh = item / a.slices, slice = item - kvh * a.slices, head0 = kvh * a.group + slice * a.G, heads = min(a.G, a.group - slice * a.G);
   __nv_bfloat16* out = a.out + (static_cast<size_t>(seq) * a.nq + head0) * kFp8D;
   int len = a.lens[seq];
+  const int held = warp == kF8CWarps ? ring.entry(a, seq, lane) : 0;     // asked for with the length
   if (len > cap) {                                       // a corrupted length: clamped and reported
     if (threadIdx.x == 0) set_status(a.status, kStatusBadIndex);
     len = cap;
@@ -593,8 +608,7 @@ decode_fp8_cluster_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid
   len = max(len, 0);
   const int n = (len + F8ClusterRing::kTile - 1) / F8ClusterRing::kTile, j = n * rank / C, count = n * (rank + 1) / C - j;
   if (warp == kF8CWarps) {
-    if (lane == 0) ring.load(a, &tm_k, &tm_v, seq, kvh, len, j, count);
-    __syncwarp();
+    ring.load(a, &tm_k, &tm_v, seq, kvh, len, j, count, 0, held, lane);
   } else {
     F8State st;
     st.begin(a.q + (static_cast<size_t>(seq) * a.nq + head0) * kFp8D, heads, a.scale_log2, lane);
@@ -667,18 +681,18 @@ static F8Grid f8_grid(int B, int nq, int nkv, int block_size, int table_width) {
 }
 
 // CTAs of an item's cluster, 0: equal shares over the GPU.  mode 1: equal shares, 2: clusters, 0: by size, the longest context being as long as the
-// block table is wide.  Measured, equal shares / clusters, us: 32 / 8 heads, 1 x 700 10.0 / 6.3, 1 x 4096 11.3 / 8.8, 1 x 16000 15.0 / 21.4, 4 x 4000
-// 13.4 / 10.7, 8 x 200 .. 2000 (64 items, clusters of 4) 12.6 / 9.8, 13 x 200 .. 2000 (104) 13.2 / 15.7, 24 x 200 .. 2000 17.0 / 20.3; 8 / 1 heads, 32 x
-// 200 .. 2000 (clusters of 8) 14.2 / 7.8; contexts of four tiles, 64 x 100 .. 500 17.2 / 15.4, 100 x 100 .. 300 18.2 / 17.6.  Clusters of 8 find no
-// place beside each other long before all SMs are taken, hence the bound of 256 CTAs (with two CTAs per SM 32 clusters took 16.1 for 7.8); clusters
-// of 16 were no faster where eight fit (1 x 3001: 7.9), and 11.5 for 6.7 where they did not.
+// block table is wide.  Measured, equal shares / clusters, us: 32 / 8 heads, 1 x 700 9.4 / 6.2, 1 x 4096 10.9 / 8.9, 1 x 16000 14.5 / 21.7, 4 x 4000
+// 12.9 / 10.5, 8 x 200 .. 2000 (64 items, clusters of 4) 11.7 / 9.7, 13 x 200 .. 2000 (104) 12.2 / 14.2, 24 x 200 .. 2000 15.5 / 23.1, 100 x 100 .. 300
+// 16.8 / 18.0; 8 / 1 heads, 32 x 200 .. 2000 (clusters of 8) 13.8 / 7.5, 64 x 100 .. 500 12.2 / 6.3.  Clusters of 8 find no place beside each other long
+// before every SM has as many CTAs as fit it: hence two per SM (where one fitted, with a third stage, 32 clusters took 16.1 for 7.8) and the
+// bound of 256.  Clusters of 16 were no faster where eight fit (1 x 3001: 7.9), and 11.5 for 6.7 where they did not.
 static int f8_cluster(long long items, int table_width, int block_size, int mode) {
   constexpr int kCtas = 256, kTilesOfOne = 4, kTiles = 8;
   if (mode == 1 || items > 65535) return 0;
   const long long tiles = (static_cast<long long>(table_width) * block_size + F8ClusterRing::kTile - 1) / F8ClusterRing::kTile;
   int c = 8;
   while (c > 1 && (items * c > kCtas || c > tiles)) c /= 2;
-  return mode == 2 || tiles <= kTilesOfOne || (c >= 4 && tiles <= kTiles * c) ? c : 0;
+  return mode == 2 || (items * c <= kCtas && (c >= 4 || tiles <= kTilesOfOne) && tiles <= kTiles * c) ? c : 0;
 }
 
 // 0: none needed.

@@ -302,7 +302,7 @@ extern "C" int forge_fp8_store(const void* qkv, long long ld, const void* qw, co
 // Pages of sequences, in order, as bf16.  A CTA takes `rows` token rows of one page of one head of K or V.  Lengths, table entry and, once the
 // latter is there, the codes are asked for one after the other; where the page goes is found out meanwhile.  Bound by memory.
 // ---------------------------------------------------------------------------------------------------------
-constexpr int kExpandThreads = 256, kExpandLoads = 8;
+constexpr int kExpandThreads = 128, kExpandLoads = 8;           // 28 x 100 .. 1024 in pages of 256 / of 64: 256 threads 19.6 / 25.3 us, 128 17.9 / 16.3, 64 18.6 / 17.4
 
 __global__ void __launch_bounds__(kExpandThreads) fp8_expand_kernel(
     const uint8_t* __restrict__ k_codes, const uint8_t* __restrict__ k_scales, const uint8_t* __restrict__ v_codes,
