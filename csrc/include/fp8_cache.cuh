@@ -58,4 +58,87 @@ __device__ __forceinline__ float2 fp8_to_float2(uint32_t codes) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
+// ---- a head in eight lanes: lane j has entries 8j .. (x) and 64 + 8j .. (y), the pairs that the rotation mixes ----
+
+// Eight consecutive bf16 values; kVec: one 16-byte access.
+template <bool kVec>
+__device__ __forceinline__ uint4 load8(const __nv_bfloat16* p) {
+  if constexpr (kVec) return *reinterpret_cast<const uint4*>(p);
+  const unsigned short* s = reinterpret_cast<const unsigned short*>(p);
+  return make_uint4(s[0] | static_cast<uint32_t>(s[1]) << 16, s[2] | static_cast<uint32_t>(s[3]) << 16, s[4] | static_cast<uint32_t>(s[5]) << 16,
+                    s[6] | static_cast<uint32_t>(s[7]) << 16);
+}
+__device__ __forceinline__ void unpack8(uint4 r, float v[8]) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = bf16_lo(w[i]);
+    v[2 * i + 1] = bf16_hi(w[i]);
+  }
+}
+__device__ __forceinline__ uint4 pack8(const float v[8]) {
+  return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+}
+// The larger one, NaN if one is.
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
+
+// A lane's norm weights of query or key heads (null: no norm).
+struct Fp8Weights {
+  float lo[8], hi[8];
+  template <bool kVec>
+  __device__ __forceinline__ void load(const __nv_bfloat16* w, int j) {
+    if (w == nullptr) return;
+    unpack8(load8<kVec>(w + 8 * j), lo);
+    unpack8(load8<kVec>(w + 64 + 8 * j), hi);
+  }
+};
+
+// RMS norm, if any, and rotation by the angles whose cos and sin stand at cs and cs + 64 (null: none), in fp32.  octet: the head's lanes.
+__device__ __forceinline__ void fp8_norm_rotate(float (&x)[8], float (&y)[8], const Fp8Weights& w, bool norm, float eps, const float* cs, unsigned octet) {
+  if (norm) {
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], fmaf(y[i], y[i], ss));
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) ss += __shfl_xor_sync(octet, ss, o);
+    const float inv = rsqrtf(ss * (1.f / kFp8D) + eps);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x[i] = x[i] * inv * w.lo[i];
+      y[i] = y[i] * inv * w.hi[i];
+    }
+  }
+  if (cs != nullptr) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 4) {
+      const float4 c = *reinterpret_cast<const float4*>(cs + i), s = *reinterpret_cast<const float4*>(cs + 64 + i);
+      rotate_pair(x[i], y[i], c.x, s.x);
+      rotate_pair(x[i + 1], y[i + 1], c.y, s.y);
+      rotate_pair(x[i + 2], y[i + 2], c.z, s.z);
+      rotate_pair(x[i + 3], y[i + 3], c.w, s.w);
+    }
+  }
+}
+
+// Codes of a head (code[0]: of x, code[1]: of y); its scale byte.
+__device__ __forceinline__ uint32_t fp8_quantise(const float (&x)[8], const float (&y)[8], unsigned octet, uint2 (&code)[2]) {
+  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) amax = max_or_nan(amax, max_or_nan(fabsf(x[i]), fabsf(y[i])));
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) amax = max_or_nan(amax, __shfl_xor_sync(octet, amax, o));
+  const uint32_t b = fp8_scale_byte(abs_bits(amax));
+  code[0] = code[1] = make_uint2(kCodesNan, kCodesNan);
+  if (b != kScaleNan) {
+    const float m = fp8_inverse_scale(b);
+    code[0] = make_uint2(fp8_pack(x[0] * m, x[1] * m, x[2] * m, x[3] * m), fp8_pack(x[4] * m, x[5] * m, x[6] * m, x[7] * m));
+    code[1] = make_uint2(fp8_pack(y[0] * m, y[1] * m, y[2] * m, y[3] * m), fp8_pack(y[4] * m, y[5] * m, y[6] * m, y[7] * m));
+  }
+  return b;
+}
+
 }  // namespace forge
