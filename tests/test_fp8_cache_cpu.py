@@ -193,3 +193,23 @@ def test_options_that_do_not_go_with_an_8_bit_cache_are_refused():
     with pytest.raises(ValueError, match="bfloat16"):
         Config("x", hf_config=preset("qwen3-0.6b"), device="cuda", dtype="float32", kv_cache_dtype="fp8")
     assert Config("x", hf_config=preset("qwen3-0.6b"), device="cuda", kv_cache_dtype="fp8").kv_cache_dtype == "fp8"
+
+
+def test_decode_steps_store_where_attention_reads():
+    """A sequence whose blocks were reserved beyond its newest token: the step's slot is in the block of that token, in every later step too."""
+    from tinyllmforge_b200 import SamplingParams
+    from tinyllmforge_b200.engine.request import Request
+    from tinyllmforge_b200.engine.step_batch import DecodeBuilder, build_decode
+    reqs = []
+    for n, table in ((5, [3, 7, 1]), (16, [2, 0]), (17, [5, 4])):
+        r = Request(list(range(n)), SamplingParams(temperature=0.0))
+        r.block_table = table
+        reqs.append(r)
+    builder = DecodeBuilder(16)
+    for i in range(12):
+        want = [r.block_table[(len(r) - 1) // 16] * 16 + (len(r) - 1) % 16 for r in reqs]
+        for step in (build_decode(reqs, 16), builder.build(reqs, 0, 0, None, None)):
+            at, size = step.offsets["slot_mapping"]
+            assert step.buf[at:at + size].tolist() == want
+        for r in reqs:
+            r.append_token(1)

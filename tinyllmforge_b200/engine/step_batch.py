@@ -201,7 +201,8 @@ def build_decode(reqs, block_size: int, step_index: int = 0, seed: int = 0,
     prev[:] = -1
     prev[:S] = [_previous(r) for r in reqs]
     sec("positions")[:S] = lens - 1
-    last_block = np.fromiter((r.block_table[-1] for r in reqs), dtype=np.int64, count=S)
+    # the newest token's place, as the attention reads it: blocks may have been reserved beyond it
+    last_block = np.fromiter((r.block_table[(len(r) - 1) // block_size] for r in reqs), dtype=np.int64, count=S)
     slots = sec("slot_mapping")
     slots[:] = -1
     slots[:S] = last_block * block_size + (lens - 1) % block_size
@@ -268,9 +269,8 @@ class DecodeBuilder:
                     to, _ = sb.offsets["block_tables"]
                     w = sb.table_width
                     for i in grew.tolist():
-                        bt = reqs[i].block_table
-                        buf[to + i * w + len(bt) - 1] = bt[-1]
-                        self.last_block[i] = bt[-1]
+                        j = (int(lens[i]) - 1) // bs
+                        buf[to + i * w + j] = self.last_block[i] = reqs[i].block_table[j]
                 o, _ = sb.offsets["slot_mapping"]
                 buf[o:o + S] = self.last_block * bs + (lens - 1) % bs
                 sb.step_index = step_index
@@ -281,5 +281,5 @@ class DecodeBuilder:
         self.key = (pad_to, table_width)
         self.sb = sb
         self.lens = np.fromiter((len(r) for r in reqs), dtype=np.int64, count=S)
-        self.last_block = np.fromiter((r.block_table[-1] for r in reqs), dtype=np.int64, count=S)
+        self.last_block = np.fromiter((r.block_table[(len(r) - 1) // bs] for r in reqs), dtype=np.int64, count=S)
         return sb
