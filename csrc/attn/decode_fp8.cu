@@ -13,7 +13,8 @@
 // bank once, and converts them in place; V^T needs no transposing load, two tokens' bytes are interleaved instead.
 //   Queries are brought to [2^14, 2^15) by a power of two per head, which keeps every bit of their bf16 down to 2^-31 of the largest entry.
 //   A value's scale 2^e goes into its weight's exponent: w_j = 2^(c q.k_j + e_j - u + 7), u a maximum of its own, and the weight into fp16 with 11 bits
-//   (half a step 2^-11, against 2^-8 of the bf16 result): a value that counts is never lost beside one with a larger scale that does not.  The
+//   (half a step 2^-11, against 2^-8 of the bf16 result): a value that counts is never lost beside one with a larger scale that does not.  Weights
+//   below 2^-21 of the largest are rounded to steps of 2^-32 of it (fp16 has no smaller ones): 2^-32 of what it adds to entries of its size.  The
 //   sum of the p_j is kept in fp32 and without that rounding.  m and u move only when they are exceeded by 8, so w_j <= 2^15 and products are
 //   rescaled rarely.
 // What is behind a sequence's last token never counts: its scores, weights and value bytes are replaced, whatever they are.
@@ -27,6 +28,8 @@
 // three, and the others ran after all the rest (256 sequences of 100 .. 1500 tokens: 82 us after an idle GPU, 116 in a row).
 // The split, few items of moderate length.  A cluster of one to eight CTAs takes an item, each a run of its tiles of 128 tokens, and they join what they
 // have through distributed shared memory: one launch, and none of the chain from kernel to kernel.
+// From the raw projection (kRaw): the step's norm, rotation and cache write happen here too, one launch less; every CTA of a cluster makes the item's queries
+// for itself, and the warp that owns the newest token puts it into its tile and into the cache.
 // Bound by memory: 258 bytes per key and KV head; few items by latency (length -> block table -> keys -> scores -> results).
 #include <algorithm>
 
@@ -43,8 +46,8 @@ constexpr float kF8Rise = 8.f;                         // how far a score may ex
 constexpr float kF8Top = 7.f;                          // weights are at most 2^(7 + 8)
 
 struct Fp8Decode {
-  const __nv_bfloat16* q;
-  const uint8_t *k_scales, *v_scales;
+  const __nv_bfloat16* q;                              // null: from the raw projection
+  uint8_t *k_codes, *v_codes, *k_scales, *v_scales;
   const int *block_tables, *lens;
   __nv_bfloat16* out;
   float *part_o, *part_ml;                             // [2 teams][G][128], [2 teams][G][2]: of a team the part that continues an item, then the one that is cut
@@ -52,7 +55,78 @@ struct Fp8Decode {
   int B, nq, nkv, group, G, slices, block_size, table_width, num_blocks;
   float scale_log2;
   unsigned* status;
+  // the step's raw projection [B][(nq + 2 nkv) * 128]: queries are normed and rotated here, and the newest token (position length - 1) stored
+  const __nv_bfloat16 *qkv, *qw, *kw;                  // norm weights may be null
+  long long ld_qkv;
+  const float* rope;                                   // [rope_rows][128] cos, sin; null: no rotation
+  int rope_rows;
+  float eps;
 };
+
+// ---- from the raw projection: what fp8_store_kernel does, with the same roundings.  Eight lanes to a head.
+__device__ __forceinline__ const float* f8_angles(const Fp8Decode& a, int len, int lane) {
+  return a.rope == nullptr ? nullptr : a.rope + static_cast<size_t>(min(max(len - 1, 0), a.rope_rows - 1)) * kFp8D + 8 * (lane & 7);
+}
+// Query heads 4 set .. of an item, bf16 [heads][128] into shared memory.
+__device__ __forceinline__ void f8_make_queries(const Fp8Decode& a, int seq, int head0, int heads, int len, int set, __nv_bfloat16* to, int lane) {
+  const int j = lane & 7, h = 4 * set + (lane >> 3);
+  if (h < heads) {
+    const __nv_bfloat16* src = a.qkv + seq * a.ld_qkv + static_cast<size_t>(head0 + h) * kFp8D + 8 * j;
+    const uint4 lo = load8<true>(src), hi = load8<true>(src + 64);
+    Fp8Weights w;
+    w.load<true>(a.qw, j);
+    float x[8], y[8];
+    unpack8(lo, x);
+    unpack8(hi, y);
+    fp8_norm_rotate(x, y, w, a.qw != nullptr, a.eps, f8_angles(a, len, lane), 0xFFu << (lane & 24));
+    *reinterpret_cast<uint4*>(to + h * kFp8D + 8 * j) = pack8(x);
+    *reinterpret_cast<uint4*>(to + h * kFp8D + 64 + 8 * j) = pack8(y);
+  }
+  __syncwarp();
+}
+// The newest token of a KV head: codes of its key and its value, 128 bytes each, then their scale bytes.  Lanes 0 .. 7 make the key's, 8 .. 15 the value's.
+constexpr int kF8Newest = 2 * kFp8D + 16;
+__device__ __forceinline__ void f8_make_newest(const Fp8Decode& a, int seq, int kvh, int len, uint8_t* to, int lane) {
+  const int j = lane & 7, is_v = lane >> 3;
+  if (is_v < 2) {
+    const __nv_bfloat16* src = a.qkv + seq * a.ld_qkv + static_cast<size_t>(a.nq + is_v * a.nkv + kvh) * kFp8D + 8 * j;
+    float x[8], y[8];
+    unpack8(load8<true>(src), x);
+    unpack8(load8<true>(src + 64), y);
+    const unsigned octet = 0xFFu << (lane & 24);
+    if (!is_v) {
+      Fp8Weights w;
+      w.load<true>(a.kw, j);
+      fp8_norm_rotate(x, y, w, a.kw != nullptr, a.eps, f8_angles(a, len, lane), octet);
+    }
+    uint2 code[2];
+    const uint32_t scale = fp8_quantise(x, y, octet, code);
+    *reinterpret_cast<uint2*>(to + is_v * kFp8D + 8 * j) = code[0];
+    *reinterpret_cast<uint2*>(to + is_v * kFp8D + 64 + 8 * j) = code[1];
+    if (j == 0) to[2 * kFp8D + is_v] = static_cast<uint8_t>(scale);
+  }
+  __syncwarp();
+}
+// By the same warp, into its row r of the tile that has just landed, whose place in the cache did not hold the token yet, and into the cache.  No other
+// warp reads that row.
+__device__ __forceinline__ void f8_put_newest(const Fp8Decode& a, int seq, int kvh, int len, const uint8_t* from, uint8_t* K, uint8_t* V, uint8_t* k_scales,
+                                              uint8_t* v_scales, int lane) {
+  const int i = lane & 7, is_v = lane >> 3, at = len - 1, r = at & 31;
+  if (is_v < 2) {
+    const uint4 piece = *reinterpret_cast<const uint4*>(from + is_v * kFp8D + 16 * i);
+    const uint8_t scale = from[2 * kFp8D + is_v];
+    *reinterpret_cast<uint4*>((is_v ? V : K) + r * kFp8D + ((i ^ (r & 7)) << 4)) = piece;
+    if (i == 0) (is_v ? v_scales : k_scales)[r] = scale;
+    const int blk = a.block_tables[static_cast<size_t>(seq) * a.table_width + at / a.block_size];
+    if (blk >= 0 && blk < a.num_blocks) {              // (reported where the tile is loaded)
+      const size_t to = (static_cast<size_t>(blk) * a.nkv + kvh) * a.block_size + at % a.block_size;
+      *reinterpret_cast<uint4*>((is_v ? a.v_codes : a.k_codes) + to * kFp8D + 16 * i) = piece;
+      if (i == 0) (is_v ? a.v_scales : a.k_scales)[to] = scale;
+    }
+  }
+  fence_proxy_async_smem();                            // a later copy into this stage comes after these writes
+  __syncwarp();
+}
 
 __device__ __forceinline__ uint32_t f8_half2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
@@ -568,11 +642,12 @@ __global__ void __launch_bounds__(32 * kF8JoinWarps, 8) decode_fp8_join_kernel(c
 constexpr int kF8CWarps = 4, kF8CStages = 2, kF8CThreads = 32 * (kF8CWarps + 1), kF8CCtasPerSm = 2;
 using F8ClusterRing = F8Ring<kF8CWarps, kF8CStages>;
 constexpr int f8_cluster_smem(int G) {
-  return 1024 + F8ClusterRing::kBytes + (kF8CWarps - 1) * F8State::kJoinFloats * 4 + G * (kFp8D + 2) * 4 + 2 * kF8CStages * 8;
+  return 1024 + F8ClusterRing::kBytes + (kF8CWarps - 1) * F8State::kJoinFloats * 4 + kF8Newest + G * (kFp8D + 2) * 4 + 2 * kF8CStages * 8;
 }
 
 // Grid (CTAs of an item, items): CTA r of C takes tiles [n r / C, n (r + 1) / C) of its item's n, and its share of the results is what all
 // of them left in their shared memory, joined.
+template <bool kRaw>
 __global__ void __launch_bounds__(kF8CThreads, kF8CCtasPerSm)
 decode_fp8_cluster_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Fp8Decode a) {
   extern __shared__ uint8_t smem_raw[];
@@ -582,7 +657,8 @@ decode_fp8_cluster_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid
   ring.codes = smem;
   ring.scales = smem + kF8CStages * 2 * F8ClusterRing::kHalf;
   float* s_join = reinterpret_cast<float*>(smem + F8ClusterRing::kBytes);
-  float* s_o = s_join + (kF8CWarps - 1) * F8State::kJoinFloats;          // [G][128]
+  uint8_t* newest = reinterpret_cast<uint8_t*>(s_join + (kF8CWarps - 1) * F8State::kJoinFloats);
+  float* s_o = reinterpret_cast<float*>(newest + kF8Newest);             // [G][128]
   float* s_ml = s_o + a.G * kFp8D;                                       // [G][2]
   ring.full = reinterpret_cast<uint64_t*>(s_ml + 2 * a.G);
   ring.empty = ring.full + kF8CStages;
@@ -611,14 +687,23 @@ decode_fp8_cluster_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid
     ring.load(a, &tm_k, &tm_v, seq, kvh, len, j, count, 0, held, lane);
   } else {
     F8State st;
-    st.begin(a.q + (static_cast<size_t>(seq) * a.nq + head0) * kFp8D, heads, a.scale_log2, lane);
+    if constexpr (kRaw) {
+      __nv_bfloat16* s_q = reinterpret_cast<__nv_bfloat16*>(s_o);        // free until results are there, after the next barrier but one
+      if (4 * warp < heads) f8_make_queries(a, seq, head0, heads, len, warp, s_q, lane);
+      if (count > 0 && j + count == n && (len - 1) % F8ClusterRing::kTile / 32 == warp) f8_make_newest(a, seq, kvh, len, newest, lane);
+      named_barrier_sync(1, 32 * kF8CWarps);
+      st.begin(s_q, heads, a.scale_log2, lane);
+    } else {
+      st.begin(a.q + (static_cast<size_t>(seq) * a.nq + head0) * kFp8D, heads, a.scale_log2, lane);
+    }
     bool ok = true;
     for (int i = 0; i < count; ++i, ring.next()) {
       const int valid = len - (j + i) * F8ClusterRing::kTile - 32 * warp;
       ok = ok && mbar_wait_parked(&ring.full[ring.s], ring.phase, a.status);
       if (valid > 0) {
-        const uint8_t* K = ring.codes + ring.s * 2 * F8ClusterRing::kHalf + 32 * warp * kFp8D;
-        const uint8_t* sc = ring.scales + ring.s * 2 * F8ClusterRing::kTile + 32 * warp;
+        uint8_t* K = ring.codes + ring.s * 2 * F8ClusterRing::kHalf + 32 * warp * kFp8D;
+        uint8_t* sc = ring.scales + ring.s * 2 * F8ClusterRing::kTile + 32 * warp;
+        if (kRaw && valid <= 32) f8_put_newest(a, seq, kvh, len, newest, K, K + F8ClusterRing::kHalf, sc, sc + F8ClusterRing::kTile, lane);
         st.take(K, K + F8ClusterRing::kHalf, sc, sc + F8ClusterRing::kTile, valid, lane);
       }
       __syncwarp();
@@ -681,18 +766,25 @@ static F8Grid f8_grid(int B, int nq, int nkv, int block_size, int table_width) {
 }
 
 // CTAs of an item's cluster, 0: equal shares over the GPU.  mode 1: equal shares, 2: clusters, 0: by size, the longest context being as long as the
-// block table is wide.  Measured, equal shares / clusters, us: 32 / 8 heads, 1 x 700 9.4 / 6.2, 1 x 4096 10.9 / 8.9, 1 x 16000 14.5 / 21.7, 4 x 4000
-// 12.9 / 10.5, 8 x 200 .. 2000 (64 items, clusters of 4) 11.7 / 9.7, 13 x 200 .. 2000 (104) 12.2 / 14.2, 24 x 200 .. 2000 15.5 / 23.1, 100 x 100 .. 300
-// 16.8 / 18.0; 8 / 1 heads, 32 x 200 .. 2000 (clusters of 8) 13.8 / 7.5, 64 x 100 .. 500 12.2 / 6.3.  Clusters of 8 find no place beside each other long
-// before every SM has as many CTAs as fit it: hence two per SM (where one fitted, with a third stage, 32 clusters took 16.1 for 7.8) and the
-// bound of 256.  Clusters of 16 were no faster where eight fit (1 x 3001: 7.9), and 11.5 for 6.7 where they did not.
+// block table is wide.  Measured, equal shares / clusters, us, 32 / 8 heads.  Clusters of 8: 1 x 700 tokens 9.4 / 6.2, 1 x 6000 12.1 / 10.9, 1 x 9000
+// 12.7 / 13.7, 1 x 16000 14.5 / 21.7, 4 x 6000 15.6 / 13.2, 4 x 9000 17.6 / 17.5.  Of 4: 8 x 200 .. 2000 11.7 / 9.7, 8 x 3000 14.8 / 12.7, 8 x 5000
+// 18.2 / 19.0.  Of 2, for which lengths that differ count more: 16 x 768 11.9 / 9.1, 16 x 1500 14.4 / 12.7, 16 x 200 .. 1500 12.2 / 12.0, 13 x 200 .. 2000
+// 12.2 / 14.2.  One CTA: 32 x 768 15.4 / 11.5, 32 x 100 .. 768 12.0 / 10.7, 32 x 100 .. 1024 13.4 / 13.2, 32 x 1500 21.9 / 22.4.  More than 256 CTAs: 100 x
+// 100 .. 300 16.8 / 18.0.  8 / 1 heads: 32 x 200 .. 2000 (clusters of 8) 13.8 / 7.5, 64 x 100 .. 500 12.2 / 6.3.  Clusters of 8 find no place beside
+// each other long before every SM has as many CTAs as fit it: hence two per SM (where one fitted, with a third stage, 32 clusters took 16.1 for
+// 7.8) and the bound of 256.  Clusters of 16 were no faster where eight fit (1 x 3001: 7.9), and 11.5 for 6.7 where they did not.
 static int f8_cluster(long long items, int table_width, int block_size, int mode) {
-  constexpr int kCtas = 256, kTilesOfOne = 4, kTiles = 8;
+  constexpr int kCtas = 256;
   if (mode == 1 || items > 65535) return 0;
   const long long tiles = (static_cast<long long>(table_width) * block_size + F8ClusterRing::kTile - 1) / F8ClusterRing::kTile;
   int c = 8;
   while (c > 1 && (items * c > kCtas || c > tiles)) c /= 2;
-  return mode == 2 || (items * c <= kCtas && (c >= 4 || tiles <= kTilesOfOne) && tiles <= kTiles * c) ? c : 0;
+  return mode == 2 || (items * c <= kCtas && tiles <= (c >= 4 ? 8 * c : 6 * c + 2)) ? c : 0;
+}
+
+// Whether a step should come from the raw projection: one launch less, against every CTA of a cluster making the item's queries.
+extern "C" int forge_decode_fp8_qkv_pays(int B, int nq, int nkv, int block_size, int table_width) {
+  return B > 0 && f8_cluster(static_cast<long long>(B) * nkv * f8_grid(B, nq, nkv, block_size, table_width).slices, table_width, block_size, 0) > 0;
 }
 
 // 0: none needed.
@@ -702,49 +794,79 @@ extern "C" long long forge_decode_fp8_scratch_floats(int B, int nq, int nkv, int
   return 2ll * z.teams * z.G * (kFp8D + 2) + 4ll * z.teams;
 }
 
+static bool f8_maps(const Fp8Decode& a, int tile, CUtensorMap* tm_k, CUtensorMap* tm_v) {
+  const uint64_t rows = static_cast<uint64_t>(a.num_blocks) * a.nkv * a.block_size;
+  const uint32_t box = static_cast<uint32_t>(std::min(a.block_size, tile));
+  return forge_make_tmap_2d(tm_k, a.k_codes, rows, kFp8D, kFp8D, box, 1) == 0 && forge_make_tmap_2d(tm_v, a.v_codes, rows, kFp8D, kFp8D, box, 1) == 0;
+}
+
+template <bool kRaw>
+static int f8_launch_clusters(const Fp8Decode& a, int C, cudaStream_t stream) {
+  CUtensorMap tm_k, tm_v;
+  if (!f8_maps(a, F8ClusterRing::kTile, &tm_k, &tm_v)) return -2;
+  FORGE_ENSURE_DYN_SMEM(decode_fp8_cluster_kernel<kRaw>, f8_cluster_smem(kF8Heads));
+  return launch_kernel_cluster_x(decode_fp8_cluster_kernel<kRaw>, dim3(C, static_cast<unsigned>(a.B * a.nkv * a.slices)), dim3(kF8CThreads), f8_cluster_smem(a.G),
+                                 stream, C, tm_k, tm_v, a) == cudaSuccess ? 0 : -5;
+}
+
+static Fp8Decode f8_operands(void* k_codes, void* k_scales, void* v_codes, void* v_scales, const int* block_tables, const int* lens, void* out,
+                             const F8Grid& z, int B, int nq, int nkv, int block_size, int table_width, int num_blocks, float scale, unsigned* status) {
+  Fp8Decode a = {};
+  a.k_codes = static_cast<uint8_t*>(k_codes); a.k_scales = static_cast<uint8_t*>(k_scales);
+  a.v_codes = static_cast<uint8_t*>(v_codes); a.v_scales = static_cast<uint8_t*>(v_scales);
+  a.block_tables = block_tables; a.lens = lens; a.out = static_cast<__nv_bfloat16*>(out);
+  a.B = B; a.nq = nq; a.nkv = nkv; a.group = nq / nkv; a.G = z.G; a.slices = z.slices; a.block_size = block_size; a.table_width = table_width; a.num_blocks = num_blocks;
+  a.scale_log2 = scale * 1.4426950408889634f; a.status = status;
+  return a;
+}
+static bool f8_shape(int nq, int nkv, int block_size) { return nkv >= 1 && nq >= nkv && nq % nkv == 0 && block_size >= 16 && (block_size & (block_size - 1)) == 0; }
+
 // q [B, nq, 128], out [B, nq * 128] bf16; a length of zero or less gives a row of zeros.  scratch: forge_decode_fp8_scratch_floats, 16-byte aligned.
 extern "C" int forge_decode_fp8(const void* q, const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales,
                                 const int* block_tables, const int* lens, void* out, float* scratch, int B, int nq, int nkv, int block_size,
                                 int table_width, int num_blocks, float scale, int mode, unsigned* status, cudaStream_t stream) {
   if (B <= 0) return 0;
-  if (nkv < 1 || nq % nkv != 0 || block_size < 16 || (block_size & (block_size - 1))) return -1;
+  if (!f8_shape(nq, nkv, block_size)) return -1;
   const F8Grid z = f8_grid(B, nq, nkv, block_size, table_width);
-  Fp8Decode a;
-  a.k_scales = static_cast<const uint8_t*>(k_scales); a.v_scales = static_cast<const uint8_t*>(v_scales);
-  a.nq = nq; a.nkv = nkv; a.group = nq / nkv; a.G = z.G; a.slices = z.slices;
-  a.block_size = block_size; a.table_width = table_width; a.num_blocks = num_blocks;
-  a.scale_log2 = scale * 1.4426950408889634f; a.status = status;
-  CUtensorMap tm_k, tm_v;
-  const uint64_t rows = static_cast<uint64_t>(num_blocks) * nkv * block_size;
-  const auto maps = [&](int tile) {
-    const uint32_t box = static_cast<uint32_t>(std::min(block_size, tile));
-    return forge_make_tmap_2d(&tm_k, k_codes, rows, kFp8D, kFp8D, box, 1) == 0 && forge_make_tmap_2d(&tm_v, v_codes, rows, kFp8D, kFp8D, box, 1) == 0;
-  };
-  const long long items = static_cast<long long>(B) * nkv * z.slices;
-  if (const int C = f8_cluster(items, table_width, block_size, mode)) {
-    a.q = static_cast<const __nv_bfloat16*>(q); a.block_tables = block_tables; a.lens = lens; a.out = static_cast<__nv_bfloat16*>(out);
-    a.part_o = a.part_ml = nullptr; a.cuts = nullptr; a.B = B;
-    if (!maps(F8ClusterRing::kTile)) return -2;
-    FORGE_ENSURE_DYN_SMEM(decode_fp8_cluster_kernel, f8_cluster_smem(kF8Heads));
-    return launch_kernel_cluster_x(decode_fp8_cluster_kernel, dim3(C, static_cast<unsigned>(items)), dim3(kF8CThreads), f8_cluster_smem(z.G), stream, C,
-                                   tm_k, tm_v, a) == cudaSuccess ? 0 : -5;
-  }
+  Fp8Decode a = f8_operands(const_cast<void*>(k_codes), const_cast<void*>(k_scales), const_cast<void*>(v_codes), const_cast<void*>(v_scales), block_tables,
+                            lens, out, z, B, nq, nkv, block_size, table_width, num_blocks, scale, status);
+  a.q = static_cast<const __nv_bfloat16*>(q);
+  if (const int C = f8_cluster(static_cast<long long>(B) * nkv * z.slices, table_width, block_size, mode)) return f8_launch_clusters<false>(a, C, stream);
   const long long tiles = (static_cast<long long>(table_width) * block_size + F8FlatRing::kTile - 1) / F8FlatRing::kTile;
   if (std::min(B, kF8Seqs) * (tiles + kF8ItemCost) * nkv * z.slices > INT32_MAX) return -1;
-  if (!maps(F8FlatRing::kTile)) return -2;
+  CUtensorMap tm_k, tm_v;
+  if (!f8_maps(a, F8FlatRing::kTile, &tm_k, &tm_v)) return -2;
   FORGE_ENSURE_DYN_SMEM(decode_fp8_kernel, kF8FlatSmem);
   a.cuts = reinterpret_cast<int4*>(scratch);
   a.part_o = scratch + 4ll * z.teams;
   a.part_ml = a.part_o + 2ll * z.teams * z.G * kFp8D;
-  for (int b0 = 0; b0 < B; b0 += kF8Seqs) {
-    a.q = static_cast<const __nv_bfloat16*>(q) + static_cast<size_t>(b0) * nq * kFp8D;
-    a.block_tables = block_tables + static_cast<size_t>(b0) * table_width; a.lens = lens + b0;
-    a.out = static_cast<__nv_bfloat16*>(out) + static_cast<size_t>(b0) * nq * kFp8D;
-    a.B = std::min(B - b0, kF8Seqs);
+  for (int left = B; left > 0; left -= kF8Seqs) {
+    a.B = std::min(left, kF8Seqs);
     if (launch_kernel(decode_fp8_kernel, dim3(z.ctas), dim3(kF8Threads), kF8FlatSmem, stream, 0, tm_k, tm_v, a) != cudaSuccess) return -5;
     if (launch_kernel(decode_fp8_join_kernel, dim3(z.teams, z.G), dim3(a.B * nkv * z.slices <= 32 ? 256 : 128), 0, stream, 0, a) != cudaSuccess) return -5;
+    a.q += static_cast<size_t>(kF8Seqs) * nq * kFp8D;
+    a.block_tables += static_cast<size_t>(kF8Seqs) * table_width;
+    a.lens += kF8Seqs;
+    a.out += static_cast<size_t>(kF8Seqs) * nq * kFp8D;
   }
   return 0;
+}
+
+// The same from the raw projection qkv [B, (nq + 2 nkv) * 128] of the sequences' newest tokens (position length - 1; rows ld apart, 16-byte aligned): queries
+// are normed and rotated, and the newest token's keys and values stored, as forge_fp8_store does, bit for bit.  Always by clusters; at most 2^16 items.
+extern "C" int forge_decode_fp8_qkv(const void* qkv, long long ld, const void* qw, const void* kw, float eps, const float* rope, int rope_rows,
+                                    void* k_codes, void* k_scales, void* v_codes, void* v_scales, const int* block_tables, const int* lens, void* out, int B,
+                                    int nq, int nkv, int block_size, int table_width, int num_blocks, float scale, unsigned* status, cudaStream_t stream) {
+  if (B <= 0) return 0;
+  if (!f8_shape(nq, nkv, block_size)) return -1;
+  const F8Grid z = f8_grid(B, nq, nkv, block_size, table_width);
+  const int C = f8_cluster(static_cast<long long>(B) * nkv * z.slices, table_width, block_size, 2);
+  if (C == 0) return -1;
+  Fp8Decode a = f8_operands(k_codes, k_scales, v_codes, v_scales, block_tables, lens, out, z, B, nq, nkv, block_size, table_width, num_blocks, scale, status);
+  a.qkv = static_cast<const __nv_bfloat16*>(qkv); a.ld_qkv = ld;
+  a.qw = static_cast<const __nv_bfloat16*>(qw); a.kw = static_cast<const __nv_bfloat16*>(kw);
+  a.eps = eps; a.rope = rope; a.rope_rows = rope_rows;
+  return f8_launch_clusters<true>(a, C, stream);
 }
 
 }  // namespace forge

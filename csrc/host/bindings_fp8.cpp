@@ -20,6 +20,10 @@ int forge_fp8_expand(const void* k_codes, const void* k_scales, const void* v_co
 int forge_decode_fp8(const void* q, const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales,
                      const int* block_tables, const int* lens, void* out, float* scratch, int B, int nq, int nkv, int block_size, int table_width,
                      int num_blocks, float scale, int mode, unsigned* status, cudaStream_t stream);
+int forge_decode_fp8_qkv(const void* qkv, long long ld, const void* qw, const void* kw, float eps, const float* rope, int rope_rows, void* k_codes,
+                         void* k_scales, void* v_codes, void* v_scales, const int* block_tables, const int* lens, void* out, int B, int nq, int nkv,
+                         int block_size, int table_width, int num_blocks, float scale, unsigned* status, cudaStream_t stream);
+int forge_decode_fp8_qkv_pays(int B, int nq, int nkv, int block_size, int table_width);
 long long forge_decode_fp8_scratch_floats(int B, int nq, int nkv, int block_size, int table_width, int mode);
 int forge_rms_norm_fp8(const void* x, void* residual, const void* w, void* codes, float* scales, int scale_ld, int rows, int H, float eps,
                        cudaStream_t stream);
@@ -65,6 +69,18 @@ const void* norm_weight(const OptTensor& w, const Tensor& with, const char* what
   return data(*w, BF, 128, what);
 }
 
+// The rotation table, if any.
+const float* angles(const OptTensor& rope, const Tensor& with, int& rows, const char* what) {
+  rows = 0;
+  if (!rope.has_value()) return nullptr;
+  TORCH_CHECK(rope->dim() == 2 && rope->size(1) == 128 && rope->size(0) >= 1, what, ": the rotation table must be [positions, 128]");
+  same_device(*rope, with, what);
+  const float* p = floats(*rope, 128, what);
+  aligned16(*rope, what);
+  rows = i32(rope->size(0));
+  return p;
+}
+
 // Returns q [T, nq, 128].
 Tensor fp8_store(const Tensor& qkv, const OptTensor& qw, const OptTensor& kw, double eps, const OptTensor& rope, const Tensor& positions,
                  const Tensor& slots, const Tensor& k_codes, const Tensor& k_scales, const Tensor& v_codes, const Tensor& v_scales, int64_t nq,
@@ -75,15 +91,8 @@ Tensor fp8_store(const Tensor& qkv, const OptTensor& qw, const OptTensor& kw, do
   const int64_t T = qkv.size(0);
   view2(qkv, BF, T, (nq + 2 * k.nkv) * 128, "fp8_store: qkv");
   TORCH_CHECK(T <= 1 || qkv.stride(0) >= qkv.size(1), "fp8_store: rows of qkv overlap");
-  const float* rp = nullptr;
-  int rope_rows = 0;
-  if (rope.has_value()) {
-    TORCH_CHECK(rope->dim() == 2 && rope->size(1) == 128 && rope->size(0) >= 1, "fp8_store: the rotation table must be [positions, 128]");
-    same_device(*rope, qkv, "fp8_store");
-    rp = floats(*rope, 128, "fp8_store: rotation table");
-    aligned16(*rope, "fp8_store: rotation table");
-    rope_rows = i32(rope->size(0));
-  }
+  int rope_rows;
+  const float* rp = angles(rope, qkv, rope_rows, "fp8_store: rotation table");
   same_device(positions, qkv, "fp8_store");
   same_device(slots, qkv, "fp8_store");
   same_device(status, qkv, "fp8_store");
@@ -143,6 +152,37 @@ Tensor decode_fp8(const Tensor& q, const Tensor& k_codes, const Tensor& k_scales
   return out;
 }
 
+// From the raw projection qkv [sequences, (nq + 2 nkv) * 128]: norm, rotation and the store of the newest token included.
+Tensor decode_fp8_qkv(const Tensor& qkv, const OptTensor& qw, const OptTensor& kw, double eps, const OptTensor& rope, const Tensor& k_codes,
+                      const Tensor& k_scales, const Tensor& v_codes, const Tensor& v_scales, const Tensor& block_tables, const Tensor& lens, int64_t nq,
+                      double scale, const Tensor& status) {
+  const Half k = cache_half(k_codes, k_scales, qkv, "decode_fp8_qkv"), v = cache_half(v_codes, v_scales, qkv, "decode_fp8_qkv");
+  TORCH_CHECK(k_codes.sizes() == v_codes.sizes(), "decode_fp8_qkv: keys and values of one shape expected");
+  TORCH_CHECK(qkv.dim() == 2 && block_tables.dim() == 2, "decode_fp8_qkv: qkv must be [sequences, (nq + 2 nkv) * 128], tables [sequences, width]");
+  const int64_t B = qkv.size(0), W = block_tables.size(1), ld = B > 1 ? qkv.stride(0) : qkv.size(1);
+  TORCH_CHECK(nq >= 1 && nq % k.nkv == 0, "decode_fp8_qkv: query heads must be a multiple of the KV heads");
+  view2(qkv, BF, B, (nq + 2 * k.nkv) * 128, "decode_fp8_qkv: qkv");
+  TORCH_CHECK(ld >= qkv.size(1) && ld % 8 == 0, "decode_fp8_qkv: rows of qkv overlap, or are not aligned to 16 bytes");
+  TORCH_CHECK(block_tables.size(0) >= B && W * k.block <= INT32_MAX, "decode_fp8_qkv: a table for every sequence expected, not too wide");
+  for (const Tensor* t : {&block_tables, &lens, &status}) same_device(*t, qkv, "decode_fp8_qkv");
+  if (B > 0) aligned16(qkv, "decode_fp8_qkv: qkv");
+  for (const OptTensor* w : {&qw, &kw})
+    if (w->has_value()) aligned16(**w, "decode_fp8_qkv: norm weights");
+  TORCH_CHECK(B * nq <= 65535, "decode_fp8_qkv: at most 65535 query heads in all: use store and attention");
+  int rope_rows;
+  const float* rp = angles(rope, qkv, rope_rows, "decode_fp8_qkv: rotation table");
+  const int* bt = ints(block_tables, B * W, "decode_fp8_qkv: tables");
+  const int* ln = ints(lens, B, "decode_fp8_qkv: lengths");
+  const void *qwp = norm_weight(qw, qkv, "decode_fp8_qkv"), *kwp = norm_weight(kw, qkv, "decode_fp8_qkv");
+  const c10::cuda::CUDAGuard guard(qkv.device());
+  Tensor out = fresh({B, nq * 128}, BF, qkv);
+  check_rc(forge_decode_fp8_qkv(qkv.data_ptr(), ld, qwp, kwp, static_cast<float>(eps), rp, rope_rows, k.codes, k.scales, v.codes, v.scales, bt, ln,
+                                out.data_ptr(), i32(B), i32(nq), i32(k.nkv), i32(k.block), i32(W), i32(k.blocks), static_cast<float>(scale),
+                                status_word(status), stream_of(qkv)),
+           "forge_decode_fp8_qkv");
+  return out;
+}
+
 // Returns the codes [rows, H] and their scales [H / 128, rows rounded up to 4].
 std::tuple<Tensor, Tensor> rms_norm_fp8(const Tensor& x, const OptTensor& residual, const Tensor& w, double eps) {
   TORCH_CHECK(x.dim() == 2 && x.size(1) >= 128 && x.size(1) % 128 == 0 && x.size(1) <= 16384,
@@ -174,5 +214,7 @@ void register_fp8(pybind11::module& m) {
   m.def("fp8_store", &fp8_store);
   m.def("fp8_expand", &fp8_expand);
   m.def("decode_fp8", &decode_fp8);
+  m.def("decode_fp8_qkv", &decode_fp8_qkv);
+  m.def("decode_fp8_qkv_pays", &forge_decode_fp8_qkv_pays);
   m.def("rms_norm_fp8", &rms_norm_fp8);
 }

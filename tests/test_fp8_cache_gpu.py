@@ -383,6 +383,178 @@ def test_blocks_beyond_four_gigabytes(ops, mode, monkeypatch):
     ops.check_status()
 
 
+# ----------------------------------------------------------------------------- decode attention from the raw projection
+def _raw_case(lens, nq, nkv, bs, seed=0):
+    """The raw projection of every sequence's newest token, whose place in the cache is NaN; positions and slots for the two ops of their own."""
+    _, kc, vc, step = _paged(lens, nq, nkv, bs, seed=seed)
+    gen = _gen(seed + 100)
+    qkv = _randn(gen, len(lens), (nq + 2 * nkv) * 128).to(BF)
+    w = [(1 + 0.2 * _randn(gen, 128)).to(BF) for _ in range(2)]
+    at = (step.context_lens - 1).clamp(min=0)
+    slots = torch.gather(step.block_tables, 1, (at // bs).long()[:, None])[:, 0] * bs + at % bs
+    slots[step.context_lens < 1] = -1
+    for c in (kc, vc):
+        for s in slots[slots >= 0].tolist():
+            c.code_bytes[s // bs, :, s % bs] = 0x7F
+            c.scales[s // bs, :, s % bs] = 255
+    return qkv, w, kc, vc, step, at, slots
+
+
+def _copy(*caches):
+    return [Fp8KVCache(c.codes.clone(), c.scales.clone()) for c in caches]
+
+
+def _two_ops(ops, qkv, w, table, kc, vc, step, at, slots, nq, nkv, do_rope=True):
+    q = ops.qk_norm_rope_store(qkv, *w, 1e-6, table, at, slots, kc, vc, nq, nkv, 128, do_rope=do_rope)
+    return ops.attention(q, kc, vc, step, SCALE)
+
+
+def _same_cache(a, b):
+    return torch.equal(a.code_bytes, b.code_bytes) and torch.equal(a.scales, b.scales)
+
+
+@pytest.mark.parametrize("lens,nq,nkv,bs", [
+    ([1], 1, 1, 16), ([1, 2, 15, 16, 17, 0, 63, 64, 65, 127], 16, 8, 256), ([17, 33, 250, 16, 1], 8, 2, 16), ([40, 96, 32], 8, 8, 32), ([513, 77], 8, 1, 64),
+    ([700, 2011, 129, 128], 32, 8, 256), ([300, 1000, 70, 2], 40, 8, 128), ([129, 640, 33], 64, 8, 256), ([50, 400], 6, 2, 64), ([255, 256, 257], 7, 1, 64),
+    ([300, 65, 2], 10, 1, 64), ([64, 513], 32, 2, 16), ([100] * 70, 5, 1, 32), ([9001, 3], 12, 4, 256), ([0, 0, 0], 4, 2, 64),
+    (list(range(1, 140, 3)), 16, 8, 128), ([5, 0, 66] * 200, 2, 1, 64),
+])
+def test_decode_from_the_raw_projection(ops, lens, nq, nkv, bs, monkeypatch):
+    """Norm, rotation and store inside the attention kernel: the bits of the two ops, in the results and in the whole cache."""
+    monkeypatch.setattr(ops, "decode_attention_mode", "chunked")
+    qkv, w, kc, vc, step, at, slots = _raw_case(lens, nq, nkv, bs)
+    table = ref.rope_table(1024, 128, 1e6, "cuda")       # shorter than the longest context: its last row is taken
+    k1, v1 = _copy(kc, vc)
+    want = _two_ops(ops, qkv, w, table, k1, v1, step, at, slots, nq, nkv)
+    got = ops.decode_attention_qkv(qkv, *w, 1e-6, table, kc, vc, step, nq, SCALE)
+    ops.check_status()
+    assert torch.equal(got, want) and not got.isnan().any()
+    assert _same_cache(kc, k1) and _same_cache(vc, v1)
+
+
+@pytest.mark.parametrize("norm,rope,ld", [(False, True, 0), (True, False, 8), (False, False, 128)])
+def test_decode_from_rows_apart_without_norm_or_rotation(ops, norm, rope, ld, monkeypatch):
+    monkeypatch.setattr(ops, "decode_attention_mode", "chunked")
+    qkv, w, kc, vc, step, at, slots = _raw_case([300, 1, 64, 1000], 8, 2, 64)
+    wide = torch.full((4, qkv.shape[1] + ld), float("nan"), dtype=BF, device="cuda")
+    wide[:, :qkv.shape[1]] = qkv
+    qkv, w = wide[:, :qkv.shape[1]], w if norm else [None, None]
+    table = ref.rope_table(1024, 128, 1e6, "cuda")
+    k1, v1 = _copy(kc, vc)
+    want = _two_ops(ops, qkv, w, table, k1, v1, step, at, slots, 8, 2, do_rope=rope)
+    got = ops.decode_attention_qkv(qkv, *w, 1e-6, table, kc, vc, step, 8, SCALE, do_rope=rope)
+    assert torch.equal(got, want) and _same_cache(kc, k1) and _same_cache(vc, v1)
+    ops.check_status()
+
+
+def test_decode_from_a_projection_that_is_not_finite(ops, monkeypatch):
+    """A newest key with an infinity spoils the query heads that read it, a newest value's NaN too; the other sequences stay as they are."""
+    monkeypatch.setattr(ops, "decode_attention_mode", "chunked")
+    qkv, w, kc, vc, step, at, slots = _raw_case([300, 70, 200], 8, 2, 64)
+    table = ref.rope_table(512, 128, 1e6, "cuda")
+    clean = ops.decode_attention_qkv(qkv, *w, 1e-6, table, *_copy(kc, vc), step, 8, SCALE).view(3, 8, 128)
+    qkv[0, 9 * 128 + 5] = float("inf")                   # the key of KV head 1
+    qkv[1, 10 * 128 + 7] = float("nan")                  # the value of KV head 0
+    k1, v1 = _copy(kc, vc)
+    want = _two_ops(ops, qkv, w, table, k1, v1, step, at, slots, 8, 2).view(3, 8, 128)
+    got = ops.decode_attention_qkv(qkv, *w, 1e-6, table, kc, vc, step, 8, SCALE).view(3, 8, 128)
+    bad = torch.zeros(3, 8, 128, dtype=torch.bool, device="cuda")
+    bad[0, 4:] = bad[1, :4] = True
+    assert torch.equal(got.isnan(), bad) and torch.equal(want.isnan(), bad)
+    assert torch.equal(got[~bad], clean[~bad]) and _same_cache(kc, k1) and _same_cache(vc, v1)
+
+
+def test_decode_from_the_raw_projection_writes_no_block_that_does_not_exist(ops, monkeypatch):
+    monkeypatch.setattr(ops, "decode_attention_mode", "chunked")
+    qkv, w, kc, vc, step, at, slots = _raw_case([300, 100, 520], 8, 2, 64)
+    table = ref.rope_table(1024, 128, 1e6, "cuda")
+    slots[1] = -1
+    k1, v1 = _copy(kc, vc)
+    want = _two_ops(ops, qkv, w, table, k1, v1, step, at, slots, 8, 2)
+    ops.check_status()
+    for bad in (-1, kc.shape[0], 2 ** 31 - 1):
+        step.block_tables[1, 1] = bad
+        k2, v2 = _copy(kc, vc)
+        got = ops.decode_attention_qkv(qkv, *w, 1e-6, table, k2, v2, step, 8, SCALE)
+        with pytest.raises(RuntimeError, match="out of range"):
+            ops.check_status()
+        assert torch.equal(got[[0, 2]], want[[0, 2]]) and _same_cache(k2, k1) and _same_cache(v2, v1)
+
+
+def test_captured_steps_from_the_raw_projection_grow_their_sequences(ops, monkeypatch):
+    """One graph, replayed for twenty tokens that cross a page, with a sequence that ends on the way: what twenty steps of the two ops leave."""
+    monkeypatch.setattr(ops, "decode_attention_mode", "chunked")
+    lens, bs, nq, nkv = [50, 1, 130], 64, 16, 8
+    _, kc, vc, step = _paged([n + 40 for n in lens], nq, nkv, bs)
+    qkv = torch.zeros(3, (nq + 2 * nkv) * 128, dtype=BF, device="cuda")
+    w = [(1 + 0.2 * _randn(_gen(1), 128)).to(BF) for _ in range(2)]
+    table = ref.rope_table(512, 128, 1e6, "cuda")
+    k1, v1 = _copy(kc, vc)
+    step.context_lens.zero_()
+    call = lambda: ops.decode_attention_qkv(qkv, *w, 1e-6, table, kc, vc, step, nq, SCALE)
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    gen = _gen(2)
+    for i in range(20):
+        now = [n + i for n in lens]
+        if i >= 12:
+            now[0] = 0
+        step.context_lens.copy_(_ints(*now))
+        qkv.copy_(_randn(gen, *qkv.shape).to(BF))
+        graph.replay()
+        at = (step.context_lens - 1).clamp(min=0)
+        slots = torch.gather(step.block_tables, 1, (at // bs).long()[:, None])[:, 0] * bs + at % bs
+        slots[step.context_lens < 1] = -1
+        want = _two_ops(ops, qkv, w, table, k1, v1, step, at, slots, nq, nkv)
+        assert torch.equal(out, want) and _same_cache(kc, k1) and _same_cache(vc, v1)
+    ops.check_status()
+
+
+def test_refusals_of_a_raw_projection(ops):
+    qkv, w, kc, vc, step, at, slots = _raw_case([40, 70], 8, 2, 64)
+    table = ref.rope_table(128, 128, 1e6, "cuda")
+
+    def attend(qkv=qkv, qw=w[0], kw=w[1], table=table, k=kc, v=vc, tables=step.block_tables, lens=step.context_lens, nq=8):
+        return ops.decode_attention_qkv(qkv, qw, kw, 1e-6, table, k, v, Step(block_tables=tables, context_lens=lens, table_width=tables.shape[1], padded_seqs=2), nq, SCALE)
+
+    attend()
+    plain = torch.zeros(kc.shape, dtype=BF, device="cuda")
+    shifted = torch.zeros(qkv.numel() + 4, dtype=BF, device="cuda")[4:].view(qkv.shape)
+    for kw in (dict(qkv=qkv.float()), dict(qkv=qkv[:, :-128]), dict(qkv=qkv[:1].expand(2, -1)), dict(qkv=qkv.cpu()), dict(qkv=shifted), dict(qkv=qkv.t().contiguous().t()),
+               dict(nq=7), dict(nq=0), dict(nq=6), dict(qw=w[0][:64]), dict(kw=w[1].float()), dict(table=table[:, :64].contiguous()), dict(table=table[:0]),
+               dict(table=table.double()), dict(v=plain), dict(v=Fp8KVCache.zeros(*kc.shape[:2], 32, 128, device="cuda")), dict(k=Fp8KVCache.zeros(*kc.shape)),
+               dict(tables=step.block_tables.long()), dict(tables=step.block_tables[:1]), dict(lens=step.context_lens.long()), dict(lens=step.context_lens[:1])):
+        with pytest.raises((RuntimeError, TypeError, ValueError)):
+            attend(**kw)
+    none = Step(block_tables=step.block_tables[:0], context_lens=step.context_lens[:0], table_width=1, padded_seqs=0)
+    assert ops.decode_attention_qkv(qkv[:0], *w, 1e-6, table, kc, vc, none, 8, SCALE).shape == (0, 1024)
+    ops.check_status()
+
+
+def test_the_rule_for_steps_from_the_raw_projection(ops, monkeypatch):
+    """Where the one op stands in for the two it gives their bits in "auto" too; over a bf16 cache the rule is what it was."""
+    monkeypatch.setattr(ops, "decode_attention_mode", "auto")
+    plain = torch.zeros(2, 8, 256, 128, dtype=BF, device="cuda")
+    cache = Fp8KVCache.zeros(2, 8, 256, 128, device="cuda")
+    most = ops.fused_qkv_max_batch
+    pays = lambda b, width, c: ops.decodes_from_projection(Step(padded_seqs=b, table_width=width), 16, c)
+    assert [pays(b, 4, plain) for b in (1, most, most + 1)] == [True, True, False]
+    assert [pays(*x, cache) for x in ((1, 4), (4, 12), (32, 4), (32, 6), (1, 100), (64, 1), (most + 1, 1))] == [True, True, True, False, False, False, False]
+    monkeypatch.setattr(ops, "decode_attention_mode", "flat")
+    assert not pays(1, 4, cache) and pays(1, 4, plain)
+    monkeypatch.setattr(ops, "decode_attention_mode", "auto")
+    for lens, nq, nkv in (([700], 16, 8), ([1000, 2000, 3], 32, 8), ([300] * 8, 8, 1)):
+        qkv, w, kc, vc, step, at, slots = _raw_case(lens, nq, nkv, 256)
+        assert ops.decodes_from_projection(step, nq, kc)
+        table = ref.rope_table(2048, 128, 1e6, "cuda")
+        want = _two_ops(ops, qkv, w, table, *_copy(kc, vc), step, at, slots, nq, nkv)
+        assert torch.equal(ops.decode_attention_qkv(qkv, *w, 1e-6, table, kc, vc, step, nq, SCALE), want)
+    ops.check_status()
+
+
 # ----------------------------------------------------------------------------- norm
 @pytest.mark.parametrize("M,H", [(1, 128), (1, 4096), (5, 384), (61, 5120), (3, 16384), (2050, 2560), (130, 1152)])
 @pytest.mark.parametrize("residual", [False, True])

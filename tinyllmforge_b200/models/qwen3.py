@@ -172,7 +172,7 @@ class Qwen3ForCausalLM:
         squares from the GEMM that updates the residual stream to the GEMM that reads it."""
         ops, layers = self.ops, self.layers
         residual, ssq_a, ssq_b = ops.embedding_ssq(batch.input_ids, self.embed_tokens.weight, self.embed_tokens.vocab_start)
-        fused_decode = (not batch.is_prefill and self.head_dim == 128 and batch.padded_seqs <= ops.fused_qkv_max_batch and not self.fp8_cache)
+        fused_decode = not batch.is_prefill and self.head_dim == 128 and ops.decodes_from_projection(batch, self.num_heads, self.kv_cache[0, 0])
         in_gemm = not self.fp8_cache and ops.qkv_rope_store_in_gemm(residual.shape[0], self.head_dim, layers[0].qkv_proj.weight, batch.is_prefill)
         for i, l in enumerate(layers):
             kc, vc = self.kv_cache[i, 0], self.kv_cache[i, 1]
@@ -198,13 +198,19 @@ class Qwen3ForCausalLM:
         """The block loop with block-scaled fp8 weights and an 8-bit cache: the norms hand 8-bit rows to qkv_proj and gate_up_proj, so
         that these need no quantiser launch of their own (two less per block)."""
         ops, residual = self.ops, None
+        fused_decode = not batch.is_prefill and hasattr(ops, "decode_attention_qkv") and ops.decodes_from_projection(batch, self.num_heads, self.kv_cache[0, 0])
         x = ops.embedding(batch.input_ids, self.embed_tokens.weight, self.embed_tokens.vocab_start)
         for i, l in enumerate(self.layers):
             kc, vc = self.kv_cache[i, 0], self.kv_cache[i, 1]
             h, residual = ops.rms_norm_fp8(x, residual, l.input_layernorm, self.eps)
-            q = ops.qk_norm_rope_store(l.qkv_proj.forward(ops, h), l.q_norm, l.k_norm, self.eps, self.rope, batch.positions,
-                                       batch.slot_mapping, kc, vc, self.num_heads, self.num_kv_heads, self.head_dim)
-            x = l.o_proj.forward(ops, ops.attention(q, kc, vc, batch, self.scale))
+            qkv = l.qkv_proj.forward(ops, h)
+            if fused_decode:
+                a = ops.decode_attention_qkv(qkv, l.q_norm, l.k_norm, self.eps, self.rope, kc, vc, batch, self.num_heads, self.scale)
+            else:
+                q = ops.qk_norm_rope_store(qkv, l.q_norm, l.k_norm, self.eps, self.rope, batch.positions, batch.slot_mapping, kc, vc, self.num_heads,
+                                           self.num_kv_heads, self.head_dim)
+                a = ops.attention(q, kc, vc, batch, self.scale)
+            x = l.o_proj.forward(ops, a)
             h, residual = ops.rms_norm_fp8(x, residual, l.post_attention_layernorm, self.eps)
             x = l.down_proj.forward(ops, l.gate_up_proj.forward_silu_mul(ops, h))
         return ops.add_rms_norm(x, residual, self.norm, self.eps)[0]
@@ -227,8 +233,8 @@ class Qwen3ForCausalLM:
         x, residual = ops.embed_norm(batch.input_ids, self.embed_tokens, layers[0].input_layernorm, self.eps)
         # small decode steps on the GPU: q/k-norm + rotation + KV store run inside the attention kernel (one launch less per
         # layer; at large batches the attention kernel is bandwidth-bound and the extra work per sequence costs more)
-        fused_decode = (not batch.is_prefill and self.head_dim == 128 and hasattr(ops, "decode_attention_qkv") and not self.fp8_cache
-                        and batch.padded_seqs <= ops.fused_qkv_max_batch)
+        fused_decode = (not batch.is_prefill and self.head_dim == 128 and hasattr(ops, "decode_attention_qkv")
+                        and ops.decodes_from_projection(batch, self.num_heads, self.kv_cache[0, 0]))
         in_gemm = (hasattr(ops, "qkv_rope_store_in_gemm") and not self.fp8_cache and getattr(layers[0].qkv_proj, "bias", None) is None
                    and ops.qkv_rope_store_in_gemm(x.shape[0], self.head_dim, layers[0].qkv_proj.weight, batch.is_prefill))
         for i, l in enumerate(layers):

@@ -345,10 +345,24 @@ class CudaOps(MixerOps, HybridOps, Fp8Ops):
             self._flat_scratch = torch.empty(need, dtype=torch.float32, device=k_cache.device)
         return ctas
 
+    def decodes_from_projection(self, batch, num_heads, k_cache) -> bool:
+        """Whether a decode step should take ``decode_attention_qkv`` rather than ``qk_norm_rope_store`` and ``attention``.  At large
+        batches the attention is bound by bandwidth, and what is saved by a launch is less than the further work per sequence
+        costs; over an 8-bit cache that is where ``attention`` would not take clusters (measured, two ops / one, us, 32 / 8 heads:
+        1 x 700 tokens 7.8 / 6.9, 4 x 3000 11.8 / 10.5, 16 x 200 8.7 / 7.4; where it does not, 32 x 1500, 24.7 / 26.5)."""
+        if batch.padded_seqs > self.fused_qkv_max_batch:
+            return False
+        if not isinstance(k_cache, Fp8KVCache):
+            return True
+        _, kv_heads, block_size, _ = k_cache.shape
+        return self.decode_attention_mode != "flat" and bool(self.C.decode_fp8_qkv_pays(batch.padded_seqs, num_heads, kv_heads, block_size, batch.table_width))
+
     def decode_attention_qkv(self, qkv, q_weight, k_weight, eps, table, k_cache, v_cache, batch, num_heads, scale, do_rope=True):
         """Decode step: attention straight from the raw qkv projection.  q/k-norm, rotation at position len - 1 and the
         KV-cache store of the step's token happen inside the attention kernel (one launch less per layer than
         ``qk_norm_rope_store`` + ``attention``).  Same partition choice as ``attention``."""
+        if isinstance(k_cache, Fp8KVCache):
+            return self.decode_attention_qkv_fp8(qkv, q_weight, k_weight, eps, table, k_cache, v_cache, batch, num_heads, scale, do_rope)
         B, D = batch.padded_seqs, k_cache.shape[3]
         out = torch.empty(B, num_heads * D, dtype=qkv.dtype, device=qkv.device)
         rope = table if do_rope else None

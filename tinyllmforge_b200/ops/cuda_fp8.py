@@ -37,6 +37,12 @@ class Fp8Ops:
         return self.C.decode_fp8(q, *self._halves(k_cache, v_cache), batch.block_tables, batch.context_lens, scale, self.status,
                                  _DECODE_MODES.get(self.decode_attention_mode, 2))
 
+    def decode_attention_qkv_fp8(self, qkv, q_weight, k_weight, eps, table, k_cache, v_cache, batch, num_heads, scale, do_rope=True):
+        """``decode_attention_qkv`` over an 8-bit cache: ``store_fp8`` at positions length - 1 and ``decode_attention_fp8`` in one, with their bits.
+        It knows only the "chunked" partition, whatever ``decode_attention_mode`` is."""
+        return self.C.decode_fp8_qkv(qkv, q_weight, k_weight, eps, table if do_rope else None, *self._halves(k_cache, v_cache), batch.block_tables,
+                                     batch.context_lens, num_heads, scale, self.status)
+
     def prefill_attention_fp8(self, q, k_cache, v_cache, batch, scale):
         """Prompts: the sequences' pages are read back and attended to by the bf16 kernels, as many sequences at a time as have
         ``expand_pages`` pages together (one at least)."""
