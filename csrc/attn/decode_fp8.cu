@@ -14,7 +14,7 @@
 //   Queries are brought to [2^14, 2^15) by a power of two per head, which keeps every bit of their bf16 down to 2^-31 of the largest entry.
 //   A value's scale 2^e goes into its weight's exponent: w_j = 2^(c q.k_j + e_j - u + 7), u a maximum of its own, and the weight into fp16 with 11 bits
 //   (half a step 2^-11, against 2^-8 of the bf16 result): a value that counts is never lost beside one with a larger scale that does not.  Weights
-//   below 2^-21 of the largest are rounded to steps of 2^-32 of it (fp16 has no smaller ones): 2^-32 of what it adds to entries of its size.  The
+//   below 2^-21 of the largest stand in steps of 2^-31 of it (fp16 has no smaller ones): nothing beside what it adds to the head.  The
 //   sum of the p_j is kept in fp32 and without that rounding.  m and u move only when they are exceeded by 8, so w_j <= 2^15 and products are
 //   rescaled rarely.
 // What is behind a sequence's last token never counts: its scores, weights and value bytes are replaced, whatever they are.
@@ -53,6 +53,7 @@ struct Fp8Decode {
   float *part_o, *part_ml;                             // [2 teams][G][128], [2 teams][G][2]: of a team the part that continues an item, then the one that is cut
   int4* cuts;                                          // [teams]: what the joining kernel has to do at the cut before a team
   int B, nq, nkv, group, G, slices, block_size, table_width, num_blocks;
+  int stages;                                          // clusters: of the ring; one where no CTA has more than a tile
   float scale_log2;
   unsigned* status;
   // the step's raw projection [B][(nq + 2 nkv) * 128]: queries are normed and rotated here, and the newest token (position length - 1) stored
@@ -347,27 +348,27 @@ struct F8State {
 
   // To and from a joining area: the same lane of another warp has the same heads and dims.  Afterwards l is the sum over the
   // tokens and not the lane's.
-  static constexpr int kJoinFloats = 32 * 32 + 6 * 4;
+  static constexpr int kOFloats = 32 * 32, kJoinFloats = kOFloats + 6 * 4;
   __device__ __forceinline__ void sum_up() {
     l[0] = f8_sum_over_tokens(l[0]);
     l[1] = f8_sum_over_tokens(l[1]);
   }
-  __device__ __forceinline__ void publish(float* area, int lane) const {
+  __device__ __forceinline__ void publish(float* area, float* maxima, int lane) const {
 #pragma unroll
     for (int i = 0; i < 32; ++i) area[i * 32 + lane] = o[i >> 2][i & 3];
     if (lane < 4) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        area[32 * 32 + 4 * h + lane] = m[h];
-        area[32 * 32 + 4 * (2 + h) + lane] = u[h];
-        area[32 * 32 + 4 * (4 + h) + lane] = l[h];
+        maxima[4 * h + lane] = m[h];
+        maxima[4 * (2 + h) + lane] = u[h];
+        maxima[4 * (4 + h) + lane] = l[h];
       }
     }
   }
-  __device__ __forceinline__ void join(const float* area, int lane) {
+  __device__ __forceinline__ void join(const float* area, const float* maxima, int lane) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {                        // (without a maximum: zeros, or NaN)
-      const float* other = area + 32 * 32 + (lane & 3);
+      const float* other = maxima + (lane & 3);
       const float m2 = other[4 * h], u2 = other[4 * (2 + h)], M = fmaxf(m[h], m2), U = fmaxf(u[h], u2);
       l[h] = l[h] * (m[h] == -INFINITY ? 0.f : ex2_approx(m[h] - M)) + other[4 * (4 + h)] * (m2 == -INFINITY ? 0.f : ex2_approx(m2 - M));
       const float f = u[h] == -INFINITY ? 0.f : ex2_approx(u[h] - U), f2 = u2 == -INFINITY ? 0.f : ex2_approx(u2 - U);
@@ -556,11 +557,12 @@ decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         if (lane == 0) mbar_arrive(&ring.empty[ring.s]);
       }
       st.sum_up();
-      if (warp > 0) st.publish(s_join + (warp - 1) * F8State::kJoinFloats, lane);
+      if (warp > 0) st.publish(s_join + (warp - 1) * F8State::kJoinFloats, s_join + (warp - 1) * F8State::kJoinFloats + F8State::kOFloats, lane);
       named_barrier_sync(1 + team, 32 * kF8Warps);
       if (warp == 0) {
 #pragma unroll
-        for (int w = 1; w < kF8Warps; ++w) st.join(s_join + (w - 1) * F8State::kJoinFloats, lane);
+        for (int w = 1; w < kF8Warps; ++w)
+          st.join(s_join + (w - 1) * F8State::kJoinFloats, s_join + (w - 1) * F8State::kJoinFloats + F8State::kOFloats, lane);
       }
       named_barrier_sync(1 + team, 32 * kF8Warps);            // the joining area is the next item's
       if (warp == 0) {
@@ -641,8 +643,10 @@ __global__ void __launch_bounds__(32 * kF8JoinWarps, 8) decode_fp8_join_kernel(c
 // ---------------------------------------------------------------------------------------------------------
 constexpr int kF8CWarps = 4, kF8CStages = 2, kF8CThreads = 32 * (kF8CWarps + 1), kF8CCtasPerSm = 2;
 using F8ClusterRing = F8Ring<kF8CWarps, kF8CStages>;
-constexpr int f8_cluster_smem(int G) {
-  return 1024 + F8ClusterRing::kBytes + (kF8CWarps - 1) * F8State::kJoinFloats * 4 + kF8Newest + G * (kFp8D + 2) * 4 + 2 * kF8CStages * 8;
+// Little of it, since the products before and after keep weights in the same SMs meanwhile: 84 -> 39 KB for one sequence of 1020 tokens took a layer of
+// 4096 x 12288 with 32 / 8 heads from 99.7 to 98.9 us.
+constexpr int f8_cluster_smem(int G, int stages) {
+  return 1024 + stages * (F8ClusterRing::kBytes / kF8CStages) + kF8Newest + G * (kFp8D + 2) * 4 + 2 * kF8CStages * 8;
 }
 
 // Grid (CTAs of an item, items): CTA r of C takes tiles [n r / C, n (r + 1) / C) of its item's n, and its share of the results is what all
@@ -655,9 +659,8 @@ decode_fp8_cluster_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cap = a.table_width * a.block_size;
   F8ClusterRing ring;
   ring.codes = smem;
-  ring.scales = smem + kF8CStages * 2 * F8ClusterRing::kHalf;
-  float* s_join = reinterpret_cast<float*>(smem + F8ClusterRing::kBytes);
-  uint8_t* newest = reinterpret_cast<uint8_t*>(s_join + (kF8CWarps - 1) * F8State::kJoinFloats);
+  ring.scales = smem + a.stages * 2 * F8ClusterRing::kHalf;
+  uint8_t* newest = ring.scales + a.stages * 2 * F8ClusterRing::kTile;
   float* s_o = reinterpret_cast<float*>(newest + kF8Newest);             // [G][128]
   float* s_ml = s_o + a.G * kFp8D;                                       // [G][2]
   ring.full = reinterpret_cast<uint64_t*>(s_ml + 2 * a.G);
@@ -710,11 +713,13 @@ decode_fp8_cluster_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid
       if (lane == 0) mbar_arrive(&ring.empty[ring.s]);
     }
     st.sum_up();
-    if (warp > 0) st.publish(s_join + (warp - 1) * F8State::kJoinFloats, lane);
+    // what a warp has takes the place of its own rows of the first stage, which no other reads and into which nothing is loaded any more
+    const auto joins = [&](int w, int half) { return reinterpret_cast<float*>(ring.codes + half * F8ClusterRing::kHalf + 32 * w * kFp8D); };
+    if (warp > 0) st.publish(joins(warp, 0), joins(warp, 1), lane);
     named_barrier_sync(1, 32 * kF8CWarps);
     if (warp == 0) {
 #pragma unroll
-      for (int w = 1; w < kF8CWarps; ++w) st.join(s_join + (w - 1) * F8State::kJoinFloats, lane);
+      for (int w = 1; w < kF8CWarps; ++w) st.join(joins(w, 0), joins(w, 1), lane);
       st.finish();
       if (C == 1) st.store(out, heads, lane);
       else st.store_part(s_o, s_ml, heads, lane);
@@ -801,11 +806,12 @@ static bool f8_maps(const Fp8Decode& a, int tile, CUtensorMap* tm_k, CUtensorMap
 }
 
 template <bool kRaw>
-static int f8_launch_clusters(const Fp8Decode& a, int C, cudaStream_t stream) {
+static int f8_launch_clusters(Fp8Decode a, int C, cudaStream_t stream) {
+  a.stages = static_cast<long long>(a.table_width) * a.block_size <= static_cast<long long>(C) * F8ClusterRing::kTile ? 1 : kF8CStages;
   CUtensorMap tm_k, tm_v;
   if (!f8_maps(a, F8ClusterRing::kTile, &tm_k, &tm_v)) return -2;
-  FORGE_ENSURE_DYN_SMEM(decode_fp8_cluster_kernel<kRaw>, f8_cluster_smem(kF8Heads));
-  return launch_kernel_cluster_x(decode_fp8_cluster_kernel<kRaw>, dim3(C, static_cast<unsigned>(a.B * a.nkv * a.slices)), dim3(kF8CThreads), f8_cluster_smem(a.G),
+  FORGE_ENSURE_DYN_SMEM(decode_fp8_cluster_kernel<kRaw>, f8_cluster_smem(kF8Heads, kF8CStages));
+  return launch_kernel_cluster_x(decode_fp8_cluster_kernel<kRaw>, dim3(C, static_cast<unsigned>(a.B * a.nkv * a.slices)), dim3(kF8CThreads), f8_cluster_smem(a.G, a.stages),
                                  stream, C, tm_k, tm_v, a) == cudaSuccess ? 0 : -5;
 }
 
