@@ -119,7 +119,7 @@ __device__ __forceinline__ void f8_put_newest(const Fp8Decode& a, int seq, int k
     *reinterpret_cast<uint4*>((is_v ? V : K) + r * kFp8D + ((i ^ (r & 7)) << 4)) = piece;
     if (i == 0) (is_v ? v_scales : k_scales)[r] = scale;
     const int blk = a.block_tables[static_cast<size_t>(seq) * a.table_width + at / a.block_size];
-    if (blk >= 0 && blk < a.num_blocks) {              // (reported where the tile is loaded)
+    if (blk >= 0 && blk < a.num_blocks && a.lens[seq] == len) {          // (reported where the tile is loaded, and the length where it was clamped)
       const size_t to = (static_cast<size_t>(blk) * a.nkv + kvh) * a.block_size + at % a.block_size;
       *reinterpret_cast<uint4*>((is_v ? a.v_codes : a.k_codes) + to * kFp8D + 16 * i) = piece;
       if (i == 0) (is_v ? a.v_scales : a.k_scales)[to] = scale;

@@ -479,6 +479,12 @@ def test_decode_from_the_raw_projection_writes_no_block_that_does_not_exist(ops,
         with pytest.raises(RuntimeError, match="out of range"):
             ops.check_status()
         assert torch.equal(got[[0, 2]], want[[0, 2]]) and _same_cache(k2, k1) and _same_cache(v2, v1)
+    step.block_tables[1, 1:] = step.block_tables[1, 0]   # a length behind the table: no place for its newest token
+    step.context_lens[1] = 64 * step.table_width + 1
+    got = ops.decode_attention_qkv(qkv, *w, 1e-6, table, kc, vc, step, 8, SCALE)
+    with pytest.raises(RuntimeError, match="out of range"):
+        ops.check_status()
+    assert torch.equal(got[[0, 2]], want[[0, 2]]) and _same_cache(kc, k1) and _same_cache(vc, v1)
 
 
 def test_captured_steps_from_the_raw_projection_grow_their_sequences(ops, monkeypatch):
