@@ -15,6 +15,7 @@ namespace forge {
 
 constexpr int kFp8D = 128;                 // entries of a head
 constexpr uint32_t kScaleNan = 255;
+constexpr uint32_t kScaleTop = 247;        // of heads whose largest entry is above 448 2^119: 2^120
 constexpr uint32_t kCodesNan = 0x7F7F7F7Fu;
 
 // |x| as an unsigned number: ordered like the values, infinities above them and NaN above those, so that a maximum keeps NaN.
@@ -124,7 +125,11 @@ __device__ __forceinline__ void fp8_norm_rotate(float (&x)[8], float (&y)[8], co
   }
 }
 
-// Codes of a head (code[0]: of x, code[1]: of y); its scale byte.
+// Of four codes those of 256 become 240, the number before it (0x78, 0x77): under the scale 2^120 256 would be infinite.
+__device__ __forceinline__ uint32_t fp8_keep_finite(uint32_t codes) { return (codes & 0x80808080u) | __vminu4(codes & 0x7F7F7F7Fu, 0x77777777u); }
+
+// Codes of a head (code[0]: of x, code[1]: of y); its scale byte.  A finite head stays finite: entries from 248 2^120 on, which are nearer to 256 than to
+// 240, are held as 240 2^120, off by no more than half a step's 2^-4 all the same.
 __device__ __forceinline__ uint32_t fp8_quantise(const float (&x)[8], const float (&y)[8], unsigned octet, uint2 (&code)[2]) {
   float amax = 0.f;
 #pragma unroll
@@ -137,6 +142,10 @@ __device__ __forceinline__ uint32_t fp8_quantise(const float (&x)[8], const floa
     const float m = fp8_inverse_scale(b);
     code[0] = make_uint2(fp8_pack(x[0] * m, x[1] * m, x[2] * m, x[3] * m), fp8_pack(x[4] * m, x[5] * m, x[6] * m, x[7] * m));
     code[1] = make_uint2(fp8_pack(y[0] * m, y[1] * m, y[2] * m, y[3] * m), fp8_pack(y[4] * m, y[5] * m, y[6] * m, y[7] * m));
+    if (b == kScaleTop) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) code[i] = make_uint2(fp8_keep_finite(code[i].x), fp8_keep_finite(code[i].y));
+    }
   }
   return b;
 }

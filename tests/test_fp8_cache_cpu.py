@@ -30,6 +30,19 @@ def test_scale_bytes_at_the_borders(top, byte):
     assert torch.equal(codes[0].float()[5], -codes[1].float()[77])
 
 
+@pytest.mark.parametrize("top,value", [(247.0, 240.0), (248.0, 240.0), (248.0 + 2 ** -16, 240.0), (255.0, 240.0), (256.0 - 2 ** -16, 240.0), (231.0, 224.0), (233.0, 240.0)])
+def test_the_largest_finite_heads_stay_finite(top, value):
+    """Entries in units of 2^120, the largest scale that 32 bits give: 256 of them would be infinite, and 240 is within half a step (2^-4)
+    of everything below."""
+    x = torch.full((2, 128), 2.0 ** 118)
+    x[0, 5], x[1, 77] = top * 2.0 ** 120, -top * 2.0 ** 120
+    codes, scales = quantize_heads(x)
+    assert scales.tolist() == [247, 247] and codes[0].float()[5] == value and codes[1].float()[77] == -value
+    v = Fp8KVCache(codes, scales).dequantize()
+    assert v.isfinite().all() and v.to(torch.bfloat16).isfinite().all()
+    oracle.check_quantised(codes, scales, x.to(F64), torch.zeros(2, dtype=F64))
+
+
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
 def test_heads_that_are_not_finite_read_back_as_nan(bad):
     x = torch.ones(3, 4, 128)

@@ -164,6 +164,36 @@ def test_store_without_norm_and_rotation_keeps_the_bits_of_the_quantiser(ops):
     ops.check_status()
 
 
+def test_the_largest_finite_heads_stay_finite(ops):
+    """Keys and values at the end of the range of bf16: the quantiser's codes, read back and attended to as finite numbers, also from the raw projection."""
+    nq, nkv, T = 2, 2, 64
+    qkv = _randn(_gen(6), T, 6 * 128).to(BF)
+    heads = qkv.view(T, 6, 128)
+    heads[:, :2] *= 2.0 ** -118                          # scores of a few units, but where a key is among the largest
+    heads[:, 2:] *= 2.0 ** 118
+    most = torch.finfo(BF).max                           # 255 2^120
+    for t, h, i, x in ((3, 2, 7, most), (3, 5, 9, -most), (40, 4, 0, 248 * 2.0 ** 120), (41, 3, 127, -249 * 2.0 ** 120), (63, 2, 64, -most), (63, 4, 1, most)):
+        heads[t, h, i] = x
+    caches = [Fp8KVCache.zeros(2, nkv, 64, 128, device="cuda") for _ in range(2)]
+    slots = torch.arange(T, device="cuda", dtype=I32)
+    table = ref.rope_table(8, 128, 1e4, "cuda")
+    q = ops.qk_norm_rope_store(qkv, None, None, 1e-6, table, slots % 8, slots, *caches, nq, nkv, 128, do_rope=False)
+    for i, c in enumerate(caches):
+        codes, scales = quantize_heads(heads[:, 2 + nkv * i:2 + nkv * (i + 1)].float())
+        assert torch.equal(c.code_bytes[0].transpose(0, 1), codes.view(torch.uint8)) and torch.equal(c.scales[0].transpose(0, 1), scales)
+        assert (scales == 247).any()
+    step = Step(is_prefill=False, num_seqs=1, padded_seqs=1, table_width=2, max_seqlen_k=T, block_tables=_ints([0, 1]), context_lens=_ints(T))
+    k, v, _ = ops.expand_kv(*caches, step.block_tables, step.context_lens, 1)
+    assert k.isfinite().all() and v.isfinite().all()
+    _check_decode(ops.attention(q[-1:].contiguous(), *caches, step, SCALE), q[-1:], *caches, step, [T])
+    again = _copy(*caches)
+    for c in again:
+        c.code_bytes[0, :, T - 1] = 0
+    got = ops.decode_attention_qkv(qkv[-1:], None, None, 1e-6, table, *again, step, nq, SCALE, do_rope=False)
+    assert got.isfinite().all() and all(_same_cache(a, b) for a, b in zip(again, caches))
+    ops.check_status()
+
+
 def test_store_reports_a_slot_behind_the_cache_and_clamps_positions(ops):
     qkv, w, table, pos, slots, caches = _store_case(6, 2, 1, 16)
     slots[2] = caches[0].shape[0] * 16

@@ -100,14 +100,16 @@ def linear_fp8_ref(x: "torch.Tensor | Fp8Rows", w: Fp8BlockWeight) -> torch.Tens
 
 def quantize_heads(x: torch.Tensor):
     """fp32 ``[..., d]`` -> (e4m3 codes ``[..., d]``, scale bytes ``[...]``) of an 8-bit KV cache: a byte b stands for 2^(b - 127), the
-    smallest power of two (not below 2^-126) with which no entry exceeds 448.  A head with an entry that is not finite has NaN in
-    every code, and 255 (NaN)."""
+    smallest power of two (not below 2^-126) with which no entry exceeds 448.  A finite head stays finite: under the largest scale, 2^120,
+    entries from 248 on are held as 240, which is within half a step of them (256 would be infinite).  A head with an entry that is
+    not finite has NaN in every code, and 255 (NaN)."""
     amax = x.abs().amax(-1)
     mantissa, exponent = torch.frexp(amax)                               # amax = mantissa 2^exponent, mantissa in [0.5, 1)
     e = exponent - 9 + (mantissa > E4M3_MAX / 512).to(exponent.dtype)
     e = torch.where(amax > 0, e, torch.full_like(e, -126)).clamp(-126, 127)
     bad = ~torch.isfinite(amax)
-    codes = torch.ldexp(x, -e[..., None]).masked_fill(bad[..., None], float("nan")).to(torch.float8_e4m3fn)
+    most = torch.where(e == 120, 240.0, E4M3_MAX)[..., None]
+    codes = torch.ldexp(x, -e[..., None]).clamp(-most, most).masked_fill(bad[..., None], float("nan")).to(torch.float8_e4m3fn)
     return codes, (e + 127).masked_fill(bad, 255).to(torch.uint8)
 
 
