@@ -44,6 +44,7 @@ constexpr int kF8Seqs = 512;                           // sequences of a launch
 constexpr int kF8Heads = 8;                            // query heads of an item
 constexpr float kF8Rise = 8.f;                         // how far a score may exceed the maximum in use
 constexpr float kF8Top = 7.f;                          // weights are at most 2^(7 + 8)
+constexpr float kF8Least = -3.402823466e38f;           // maximum before any score.  Finite, so that a score of -infinity (masked, or beyond 32 bits) has no weight beside it
 
 struct Fp8Decode {
   const __nv_bfloat16* q;                              // null: from the raw projection
@@ -231,7 +232,7 @@ struct F8State {
     for (int i = 0; i < 16; ++i) qh[i] = f8_half2(bf16_lo(w[i]) * up, bf16_hi(w[i]) * up);
     qf[0] = scale_log2 / __shfl_sync(0xffffffffu, up, 8 * quad);
     qf[1] = scale_log2 / __shfl_sync(0xffffffffu, up, 8 * quad + 4);
-    m[0] = m[1] = u[0] = u[1] = -INFINITY;
+    m[0] = m[1] = u[0] = u[1] = kF8Least;
     l[0] = l[1] = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
@@ -311,7 +312,7 @@ struct F8State {
         }
       }
     }
-    // ---- weights.  A token that counts has given each maximum a value, or its score is not finite and the result is NaN.
+    // ---- weights.  A score that is NaN or +infinity makes the result NaN; where all are -infinity the sums stay zero, and so does the result.
     uint32_t p[4];
     {
       const float u0 = u[0] - kF8Top, u1 = u[1] - kF8Top;
@@ -367,11 +368,11 @@ struct F8State {
   }
   __device__ __forceinline__ void join(const float* area, const float* maxima, int lane) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {                        // (without a maximum: zeros, or NaN)
+    for (int h = 0; h < 2; ++h) {                        // (without a score: zeros)
       const float* other = maxima + (lane & 3);
       const float m2 = other[4 * h], u2 = other[4 * (2 + h)], M = fmaxf(m[h], m2), U = fmaxf(u[h], u2);
-      l[h] = l[h] * (m[h] == -INFINITY ? 0.f : ex2_approx(m[h] - M)) + other[4 * (4 + h)] * (m2 == -INFINITY ? 0.f : ex2_approx(m2 - M));
-      const float f = u[h] == -INFINITY ? 0.f : ex2_approx(u[h] - U), f2 = u2 == -INFINITY ? 0.f : ex2_approx(u2 - U);
+      l[h] = l[h] * (m[h] == kF8Least ? 0.f : ex2_approx(m[h] - M)) + other[4 * (4 + h)] * (m2 == kF8Least ? 0.f : ex2_approx(m2 - M));
+      const float f = u[h] == kF8Least ? 0.f : ex2_approx(u[h] - U), f2 = u2 == kF8Least ? 0.f : ex2_approx(u2 - U);
 #pragma unroll
       for (int k = 0; k < 16; ++k) {
         float& v = o[k >> 1][2 * (k & 1) + h];
@@ -385,7 +386,7 @@ struct F8State {
   __device__ __forceinline__ void finish() {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const float f = l[h] == 0.f ? 0.f : 1.f / l[h] * exp2f(u[h] - m[h] - kF8Top);        // (no tokens: no maxima either)
+      const float f = l[h] == 0.f ? 0.f : 1.f / l[h] * exp2f(u[h] - m[h] - kF8Top);        // (no score: zeros)
 #pragma unroll
       for (int k = 0; k < 16; ++k) o[k >> 1][2 * (k & 1) + h] *= f;
     }
@@ -602,7 +603,7 @@ __global__ void __launch_bounds__(32 * kF8JoinWarps, 8) decode_fp8_join_kernel(c
   const int parts = cut.x, kvh = cut.z / a.slices, slice = cut.z - kvh * a.slices;
   if (parts == 0 || head >= min(a.G, a.group - slice * a.G)) return;
   const auto slot = [&](int i) { return static_cast<size_t>(i == 0 ? 2 * (me - 1) + 1 : 2 * (me + i - 1)) * a.G + head; };
-  float M = -INFINITY, L = 0.f;                          // of the warp's parts
+  float M = kF8Least, L = 0.f;                           // of the warp's parts
   float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
   for (int i = warp; i < parts; i += warps) {
@@ -610,7 +611,7 @@ __global__ void __launch_bounds__(32 * kF8JoinWarps, 8) decode_fp8_join_kernel(c
     const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * p);
     const float4 v = *reinterpret_cast<const float4*>(a.part_o + p * kFp8D + 4 * lane);
     const float m = fmaxf(M, ml.x);
-    const float keep = M == -INFINITY ? 0.f : ex2_approx(M - m), f = (ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - m)) * ml.y;
+    const float keep = M == kF8Least ? 0.f : ex2_approx(M - m), f = (ml.x == kF8Least ? 0.f : ex2_approx(ml.x - m)) * ml.y;
     M = m;
     L = L * keep + f;
     O.x = O.x * keep + f * v.x;
@@ -628,7 +629,7 @@ __global__ void __launch_bounds__(32 * kF8JoinWarps, 8) decode_fp8_join_kernel(c
   O = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int i = 0; i < n; ++i) {
     const float4 v = s_o[i][lane];
-    const float f = s_ml[i].x == -INFINITY ? 0.f : ex2_approx(s_ml[i].x - M);
+    const float f = s_ml[i].x == kF8Least ? 0.f : ex2_approx(s_ml[i].x - M);
     L += f * s_ml[i].y;
     O.x += f * v.x; O.y += f * v.y; O.z += f * v.z; O.w += f * v.w;
   }
@@ -731,14 +732,14 @@ decode_fp8_cluster_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid
   const int pieces = heads * (kFp8D / 4);                // four dims of a head each
   for (int i = pieces * rank / C + threadIdx.x; i < pieces * (rank + 1) / C; i += kF8CThreads) {
     const int head = i / (kFp8D / 4);
-    float M = -INFINITY, L = 0.f;
+    float M = kF8Least, L = 0.f;
     float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
     const uint32_t ml_at = smem_u32(s_ml + 2 * head), o_at = smem_u32(s_o + 4 * i);
     for (int c = 0; c < C; ++c) M = fmaxf(M, ld_dsmem_f2(dsmem_addr(ml_at, c)).x);
     for (int c = 0; c < C; ++c) {
       const float2 ml = ld_dsmem_f2(dsmem_addr(ml_at, c));
       const float4 v = ld_dsmem_f4(dsmem_addr(o_at, c));
-      const float f = (ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - M)) * ml.y;
+      const float f = (ml.x == kF8Least ? 0.f : ex2_approx(ml.x - M)) * ml.y;
       L += f;
       O.x = fmaf(f, v.x, O.x);
       O.y = fmaf(f, v.y, O.y);

@@ -335,6 +335,26 @@ def test_decode_keeps_nan_where_it_belongs(ops, mode, monkeypatch):
 
 
 @pytest.mark.parametrize("mode", ["flat", "chunked"])
+def test_decode_of_scores_below_the_range_of_32_bits(ops, mode, monkeypatch):
+    """Keys so large that their scores are minus infinity have no weight, whether a warp's tokens are all of that kind or some."""
+    monkeypatch.setattr(ops, "decode_attention_mode", mode)
+    lens, gone = [33, 64, 300, 40, 700], [range(32, 33), range(0, 32), range(0, 128), range(5, 6), range(640, 700)]
+    q, kc, vc, step = _paged(lens, 8, 2, 64)
+    q.abs_().clamp_(min=0.5)
+    for i, tokens in enumerate(gone):
+        for t in tokens:
+            b = step.block_tables[i, t // 64].long()
+            kc.code_bytes[b, :, t % 64] = 0xF7           # -240 2^120: at most -64 240 2^120 / sqrt(128) with the query
+            kc.scales[b, :, t % 64] = 247
+    got = ops.attention(q, kc, vc, step, SCALE).to(F64).view(len(lens), 8, 128)
+    for i, n in enumerate(lens):
+        left = [t for t in range(n) if t not in gone[i]]
+        want, allowed = oracle.attention(q[i], *(oracle.sequence(c, step.block_tables[i], n)[:, left] for c in (kc, vc)), SCALE)
+        assert ((got[i] - want).abs() <= allowed).all(), f"sequence {i}"
+    ops.check_status()
+
+
+@pytest.mark.parametrize("mode", ["flat", "chunked"])
 def test_decode_reports_lengths_and_blocks_that_do_not_exist(ops, mode, monkeypatch):
     monkeypatch.setattr(ops, "decode_attention_mode", mode)
     lens = [300, 100, 520]
