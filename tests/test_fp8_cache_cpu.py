@@ -1,5 +1,7 @@
 """Keys, values and normed rows in 8 bits on the PyTorch op set: formats, refusals, ops against 64 bits, the engine."""
 import random
+import types
+import weakref
 
 import fp8_oracle as oracle
 import pytest
@@ -226,3 +228,38 @@ def test_decode_steps_store_where_attention_reads():
             assert step.buf[at:at + size].tolist() == want
         for r in reqs:
             r.append_token(1)
+
+
+def _prompt_ops(tokens, bs):
+    """The prompt attention of the GPU over stand-ins of its kernels; ``most``: pages that were read back and alive at once, ``portions``: (sequences, pages)."""
+    from tinyllmforge_b200.ops.cuda_fp8 import Fp8Ops
+    ops, alive = Fp8Ops(), weakref.WeakSet()
+    ops.expand_tokens, ops.status, ops.portions, ops.most = tokens, None, [], 0
+
+    def expand(kc, ks, vc, vs, tables, lens, pages, status):
+        out = tuple(torch.empty(pages, 1, bs, 128, dtype=torch.bfloat16) for _ in range(2))
+        alive.update(out)
+        ops.most = max(ops.most, sum(t.shape[0] for t in alive))
+        return (*out, tables.clone())
+
+    def attend(q, k, v, cu, lens, tables, out, n, *rest):
+        ops.portions.append((n, k.shape[0]))
+
+    ops.C = types.SimpleNamespace(fp8_expand=expand, prefill_attention=attend)
+    return ops
+
+
+def test_a_portions_pages_are_freed_before_the_next_is_read_back():
+    """A step of several portions holds the pages of one at a time: that much is in the peak that the cache is sized after."""
+    bs, lens = 16, [64, 48, 16, 100, 33, 0, 128]
+    ops = _prompt_ops(128, bs)
+    cache = Fp8KVCache.zeros(4, 1, bs, 128)
+
+    class B:
+        num_seqs, max_seqlen_q, key_lens = len(lens), 1, lens
+        block_tables, context_lens = torch.zeros(len(lens), 8, dtype=torch.int32), torch.tensor(lens)
+        cu_seqlens_q = torch.arange(len(lens) + 1)
+
+    ops.prefill_attention_fp8(torch.zeros(len(lens), 1, 128, dtype=torch.bfloat16), cache, cache, B, 1.0)
+    assert ops.portions == [(3, 8), (1, 7), (2, 3), (1, 8)]
+    assert ops.most == 2 * 8                             # keys and values

@@ -45,7 +45,7 @@ class Fp8Ops:
 
     def prefill_attention_fp8(self, q, k_cache, v_cache, batch, scale):
         """Prompts: the sequences' pages are read back and attended to by the bf16 kernels, as many sequences at a time as have
-        ``expand_pages`` pages together (one at least)."""
+        ``expand_pages`` pages together (one at least).  One portion's pages are held at a time."""
         T, H, D = q.shape
         out = torch.empty(T, H * D, dtype=q.dtype, device=q.device)
         bs, lens = k_cache.shape[2], getattr(batch, "key_lens", None)
@@ -62,6 +62,7 @@ class Fp8Ops:
                 k, v, tables = self.expand_kv(k_cache, v_cache, batch.block_tables[part], batch.context_lens[part], pages)
                 self.C.prefill_attention(q, k, v, batch.cu_seqlens_q[begin:end + 1], batch.context_lens[part], tables, out, end - begin,
                                          batch.max_seqlen_q, scale, self.status)
+                del k, v, tables                  # before the next portion asks for its own
             begin = end
         return out
 
