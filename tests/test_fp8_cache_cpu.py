@@ -263,3 +263,33 @@ def test_a_portions_pages_are_freed_before_the_next_is_read_back():
     ops.prefill_attention_fp8(torch.zeros(len(lens), 1, 128, dtype=torch.bfloat16), cache, cache, B, 1.0)
     assert ops.portions == [(3, 8), (1, 7), (2, 3), (1, 8)]
     assert ops.most == 2 * 8                             # keys and values
+
+
+@pytest.mark.parametrize("budget,max_len,seqs,bs,pages", [
+    (16384, 9000, 512, 256, 64 - 36),                    # the warm-up has one prompt of 9000 tokens, later portions up to 64 pages
+    (16384, 4096, 512, 256, 0), (16384, 9000, 1, 256, 0),
+    (16384, 40960, 512, 256, 160 - 64), (2048, 100, 512, 64, 32 - 32), (2048, 90, 3, 64, 0), (1000, 700, 512, 16, 62 - 44),
+    (1000, 300, 512, 256, 3 - 2),                        # at most 3 pages together: one prompt of two in the warm-up, 300 and 200 tokens later
+])
+def test_the_cache_leaves_room_for_the_largest_portion_read_back(budget, max_len, seqs, bs, pages):
+    """Beyond what the warm-up has read back: the most that any step of this configuration does."""
+    from tinyllmforge_b200.engine.worker import warmup_lengths
+    cfg = Config("x", hf_config=preset("tiny", max_position_embeddings=max_len), device="cpu", kvcache_block_size=bs, max_model_len=max_len,
+                 max_num_batched_tokens=budget, max_num_seqs=seqs, chunked_prefill=True, kv_cache_dtype="fp8")
+    model = _llm().worker.model
+    warm = warmup_lengths(cfg)
+    assert model.expansion_beyond(cfg, warm) == model.expansion_bytes(pages * bs)
+    rng, cache = random.Random(0), Fp8KVCache.zeros(1, 1, bs, 128)
+
+    def most(lens):
+        ops = _prompt_ops(budget, bs)
+        step = types.SimpleNamespace(num_seqs=len(lens), max_seqlen_q=1, key_lens=lens, block_tables=torch.zeros(len(lens), 1, dtype=torch.int32),
+                                     context_lens=torch.tensor(lens), cu_seqlens_q=torch.arange(len(lens) + 1))
+        ops.prefill_attention_fp8(torch.zeros(len(lens), 1, 128, dtype=torch.bfloat16), cache, cache, step, 1.0)
+        return max(p for _, p in ops.portions)
+
+    for _ in range(50):
+        lens = [rng.choice((1, max_len, rng.randint(1, max_len))) for _ in range(rng.randint(1, min(seqs, 40)))]
+        assert most(lens) <= most(warm) + pages
+    model.fp8_cache = False
+    assert model.expansion_beyond(cfg, warm) == 0

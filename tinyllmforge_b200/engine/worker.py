@@ -60,6 +60,12 @@ def graph_buckets(max_num_seqs: int) -> list[int]:
     return [b for b in (1, 2, 4, 8) if b <= top] + list(range(16, top + 1, 16))
 
 
+def warmup_lengths(cfg: Config) -> list[int]:
+    """The prompts of the warm-up: as many of the longest as one step's token budget holds (with chunked prefill a step never exceeds it)."""
+    longest = min(cfg.max_model_len, cfg.max_num_batched_tokens)
+    return [longest] * max(1, min(cfg.max_num_batched_tokens // longest, cfg.max_num_seqs))
+
+
 class Worker:
     def __init__(self, config: Config, rank: int, tp: TPGroup):
         self.config, self.rank, self.tp = config, rank, tp
@@ -123,14 +129,11 @@ class Worker:
     def _warmup(self) -> None:
         """One full-budget prefill so the allocator's peak reflects the largest step
         (tinyvllm/engine/model_runner.py:108-116)."""
-        cfg = self.config
-        seq_len = min(cfg.max_model_len, cfg.max_num_batched_tokens)      # chunked prefill: a step never exceeds the budget
-        n = max(1, min(cfg.max_num_batched_tokens // seq_len, cfg.max_num_seqs))
         from .request import Request
         reqs = []
-        nblk = (seq_len + self.block_size - 1) // self.block_size
-        for i in range(n):
-            r = Request([0] * seq_len)
+        for i, n in enumerate(warmup_lengths(self.config)):
+            nblk = (n + self.block_size - 1) // self.block_size
+            r = Request([0] * n)
             r.block_table = list(range(i * nblk, (i + 1) * nblk))
             r.state_slot = i if self.num_slots else -1
             reqs.append(r)
@@ -143,8 +146,8 @@ class Worker:
         if cfg.num_kvcache_blocks <= 0:
             if self.is_cuda:
                 # temporary cache just large enough for the warm-up prefill
-                n_tmp = max(1, min(cfg.max_num_batched_tokens // min(cfg.max_model_len, cfg.max_num_batched_tokens), cfg.max_num_seqs)) * self.table_width
-                self.model.bind_cache(n_tmp, self.block_size, self.num_slots)
+                warm = warmup_lengths(cfg)
+                self.model.bind_cache(len(warm) * self.table_width, self.block_size, self.num_slots)
                 torch.cuda.reset_peak_memory_stats()
                 self._warmup()
                 torch.cuda.synchronize()
@@ -154,8 +157,7 @@ class Worker:
                 stats = torch.cuda.memory_stats()
                 peak, cur = stats["allocated_bytes.all.peak"], stats["allocated_bytes.all.current"]
                 budget = int(total * cfg.gpu_memory_utilization) - (total - free) - (peak - cur) - self.num_slots * self.model.state_bytes()
-                # chunked prefill: a late portion of a long prompt sees more keys than the warm-up's whole prompts did
-                budget -= self.model.expansion_bytes(max(0, cfg.max_model_len - cfg.max_num_batched_tokens))
+                budget -= self.model.expansion_beyond(cfg, warm)
                 # a model whose layers are all recurrent pages nothing: the blocks then only bound the tokens of live requests
                 n = budget // block_bytes if block_bytes else cfg.max_num_seqs * self.table_width
                 if budget <= 0:

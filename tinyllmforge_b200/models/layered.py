@@ -79,6 +79,11 @@ class LayeredDecoder:
         """Largest workspace that ``tokens`` cached keys take when a portion of a prompt sees them."""
         return tokens * max((l.mix.expansion_bytes() for l in self.layers), default=0)
 
+    def expansion_beyond(self, config, warm: list[int]) -> int:
+        """How much larger that workspace can be than in the warm-up with prompts ``warm``: with chunked prefill a late portion of a long prompt sees
+        more keys than the warm-up's whole prompts did."""
+        return self.expansion_bytes(max(0, config.max_model_len - config.max_num_batched_tokens))
+
     def bind_cache(self, num_blocks: int, block_size: int, num_slots: int) -> None:
         """Every layer run has a cache or state of its own, or borrows an earlier layer's; all share block and slot numbers."""
         self.memory, latest = [], {}

@@ -25,6 +25,7 @@ import torch
 
 from ..config import ModelConfig
 from ..ops import ref as ref_ops
+from ..ops.cuda_fp8 import expand_portions, largest_portion
 from ..ops.quant import Fp8BlockWeight, Fp8KVCache
 from ..parallel.comm import TPGroup
 from ..parallel.tp_layers import (MergedColumnParallelLinear, ParallelLMHead, QKVParallelLinear,
@@ -122,6 +123,14 @@ class Qwen3ForCausalLM:
     def expansion_bytes(self, tokens: int) -> int:
         """Workspace of ``tokens`` cached keys that a prompt's attention reads back from 8 bits."""
         return 2 * tokens * self.num_kv_heads * self.head_dim * self.norm.element_size() if self.fp8_cache else 0
+
+    def expansion_beyond(self, config, warm: list[int]) -> int:
+        """How much larger that workspace can be than in the warm-up with prompts ``warm``: the largest portion that any step reads back
+        against the warm-up's largest."""
+        bs, tokens = config.kvcache_block_size, config.max_num_batched_tokens
+        most = largest_portion(config.max_num_seqs, config.max_model_len, bs, tokens)
+        held = max(pages for _, _, pages in expand_portions(warm, bs, tokens))
+        return self.expansion_bytes((most - held) * bs)
 
     def bind_cache(self, num_blocks: int, block_size: int, num_slots: int = 0) -> None:
         if self.fp8_cache:

@@ -11,6 +11,30 @@ from .quant import Fp8KVCache, Fp8Rows
 _DECODE_MODES = {"auto": 0, "flat": 1, "chunked": 2}
 
 
+def expand_pages(tokens: int, block_size: int) -> int:
+    """Pages that a portion of several sequences has at most, for a step's budget of ``tokens``."""
+    return max(1, tokens // block_size)
+
+
+def expand_portions(lens, block_size: int, tokens: int):
+    """(begin, end, pages): the sequences, in order, that a prompt's attention reads back together: as many as have ``expand_pages`` pages,
+    one at least."""
+    begin = 0
+    while begin < len(lens):
+        end, pages = begin, 0
+        while end < len(lens) and (end == begin or pages + -(-lens[end] // block_size) <= expand_pages(tokens, block_size)):
+            pages += -(-lens[end] // block_size)
+            end += 1
+        yield begin, end, pages
+        begin = end
+
+
+def largest_portion(max_seqs: int, max_len: int, block_size: int, tokens: int) -> int:
+    """Pages of the largest portion of any step of up to ``max_seqs`` sequences of up to ``max_len`` tokens."""
+    one = -(-max_len // block_size)
+    return max(one, min(expand_pages(tokens, block_size), max_seqs * one))
+
+
 class Fp8Ops:
     """Mixed into ``CudaOps`` (uses its ``C``, ``status``, ``device`` and ``num_sms``)."""
 
@@ -44,30 +68,21 @@ class Fp8Ops:
                                      batch.context_lens, num_heads, scale, self.status)
 
     def prefill_attention_fp8(self, q, k_cache, v_cache, batch, scale):
-        """Prompts: the sequences' pages are read back and attended to by the bf16 kernels, as many sequences at a time as have
-        ``expand_pages`` pages together (one at least).  One portion's pages are held at a time."""
+        """Prompts: the sequences' pages are read back and attended to by the bf16 kernels, the pages of one portion
+        (``expand_portions``) at a time."""
         T, H, D = q.shape
         out = torch.empty(T, H * D, dtype=q.dtype, device=q.device)
         bs, lens = k_cache.shape[2], getattr(batch, "key_lens", None)
         if lens is None:                          # lengths unknown on the host: as long as the table is wide
             lens = [min(batch.max_seqlen_k, batch.block_tables.shape[1] * bs)] * batch.num_seqs
-        begin = 0
-        while begin < batch.num_seqs:
-            end, pages = begin, 0
-            while end < batch.num_seqs and (end == begin or pages + -(-lens[end] // bs) <= self.expand_pages(bs)):
-                pages += -(-lens[end] // bs)
-                end += 1
+        for begin, end, pages in expand_portions(lens[:batch.num_seqs], bs, self.expand_tokens):
             part = slice(begin, end)
             if pages:                             # (sequences without keys have no queries either)
                 k, v, tables = self.expand_kv(k_cache, v_cache, batch.block_tables[part], batch.context_lens[part], pages)
                 self.C.prefill_attention(q, k, v, batch.cu_seqlens_q[begin:end + 1], batch.context_lens[part], tables, out, end - begin,
                                          batch.max_seqlen_q, scale, self.status)
                 del k, v, tables                  # before the next portion asks for its own
-            begin = end
         return out
-
-    def expand_pages(self, block_size: int) -> int:
-        return max(1, self.expand_tokens // block_size)
 
     # ------------------------------------------------------------------ norms with 8-bit rows
     def takes_fp8_rows(self, weight, rows: int) -> bool:
