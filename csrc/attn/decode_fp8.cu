@@ -755,6 +755,8 @@ decode_fp8_cluster_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid
 
 extern "C" int forge_make_tmap_2d(CUtensorMap* tm, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows, int elem_bytes);
 
+static bool f8_shape(int nq, int nkv, int block_size) { return nkv >= 1 && nq >= nkv && nq % nkv == 0 && block_size >= 16 && (block_size & (block_size - 1)) == 0; }
+
 // Grid of a launch of up to 512 sequences; G: query heads of an item.
 struct F8Grid {
   int slices, G, ctas, teams;
@@ -788,13 +790,15 @@ static int f8_cluster(long long items, int table_width, int block_size, int mode
   return mode == 2 || (items * c <= kCtas && tiles <= (c >= 4 ? 8 * c : 6 * c + 2)) ? c : 0;
 }
 
-// Whether a step should come from the raw projection: one launch less, against every CTA of a cluster making the item's queries.
+// Whether a step should come from the raw projection: one launch less, against every CTA of a cluster making the item's queries.  -1: no such shape.
 extern "C" int forge_decode_fp8_qkv_pays(int B, int nq, int nkv, int block_size, int table_width) {
+  if (!f8_shape(nq, nkv, block_size)) return -1;
   return B > 0 && f8_cluster(static_cast<long long>(B) * nkv * f8_grid(B, nq, nkv, block_size, table_width).slices, table_width, block_size, 0) > 0;
 }
 
 // 0: none needed.
 extern "C" long long forge_decode_fp8_scratch_floats(int B, int nq, int nkv, int block_size, int table_width, int mode) {
+  if (!f8_shape(nq, nkv, block_size)) return 0;
   const F8Grid z = f8_grid(B, nq, nkv, block_size, table_width);
   if (f8_cluster(static_cast<long long>(B) * nkv * z.slices, table_width, block_size, mode)) return 0;
   return 2ll * z.teams * z.G * (kFp8D + 2) + 4ll * z.teams;
@@ -826,7 +830,6 @@ static Fp8Decode f8_operands(void* k_codes, void* k_scales, void* v_codes, void*
   a.scale_log2 = scale * 1.4426950408889634f; a.status = status;
   return a;
 }
-static bool f8_shape(int nq, int nkv, int block_size) { return nkv >= 1 && nq >= nkv && nq % nkv == 0 && block_size >= 16 && (block_size & (block_size - 1)) == 0; }
 
 // q [B, nq, 128], out [B, nq * 128] bf16; a length of zero or less gives a row of zeros.  scratch: forge_decode_fp8_scratch_floats, 16-byte aligned.
 extern "C" int forge_decode_fp8(const void* q, const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales,

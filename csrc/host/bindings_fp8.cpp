@@ -183,6 +183,12 @@ Tensor decode_fp8_qkv(const Tensor& qkv, const OptTensor& qw, const OptTensor& k
   return out;
 }
 
+bool decode_fp8_qkv_pays(int64_t B, int64_t nq, int64_t nkv, int64_t block, int64_t W) {
+  const int pays = forge_decode_fp8_qkv_pays(i32(B), i32(nq), i32(nkv), i32(block), i32(W));
+  TORCH_CHECK(pays >= 0, "decode_fp8_qkv_pays: query heads must be a multiple of the KV heads, block_size a power of two from 16 on; got ", nq, ", ", nkv, ", ", block);
+  return pays != 0;
+}
+
 // Returns the codes [rows, H] and their scales [H / 128, rows rounded up to 4].
 std::tuple<Tensor, Tensor> rms_norm_fp8(const Tensor& x, const OptTensor& residual, const Tensor& w, double eps) {
   TORCH_CHECK(x.dim() == 2 && x.size(1) >= 128 && x.size(1) % 128 == 0 && x.size(1) <= 16384,
@@ -215,6 +221,6 @@ void register_fp8(pybind11::module& m) {
   m.def("fp8_expand", &fp8_expand);
   m.def("decode_fp8", &decode_fp8);
   m.def("decode_fp8_qkv", &decode_fp8_qkv);
-  m.def("decode_fp8_qkv_pays", &forge_decode_fp8_qkv_pays);
+  m.def("decode_fp8_qkv_pays", &decode_fp8_qkv_pays);
   m.def("rms_norm_fp8", &rms_norm_fp8);
 }

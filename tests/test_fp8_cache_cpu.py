@@ -293,3 +293,15 @@ def test_the_cache_leaves_room_for_the_largest_portion_read_back(budget, max_len
         assert most(lens) <= most(warm) + pages
     model.fp8_cache = False
     assert model.expansion_beyond(cfg, warm) == 0
+
+
+def test_the_rule_for_steps_from_the_raw_projection_refuses_heads_that_do_not_go_together():
+    _C = pytest.importorskip("tinyllmforge_b200._C")
+    from tinyllmforge_b200.ops.cuda import CudaOps
+    ops = object.__new__(CudaOps)
+    ops.C, ops.fused_qkv_max_batch, ops.decode_attention_mode = _C, 32, "auto"
+    step = types.SimpleNamespace(padded_seqs=1, table_width=2)
+    assert ops.decodes_from_projection(step, 16, Fp8KVCache.zeros(2, 8, 64, 128))
+    for heads, kv_heads, block in ((4, 8, 64), (0, 1, 64), (7, 2, 64), (4, 0, 64), (-8, 8, 64), (8, 8, 24), (8, 8, 8)):
+        with pytest.raises(RuntimeError, match="decode_fp8_qkv_pays"):
+            ops.decodes_from_projection(step, heads, Fp8KVCache.zeros(2, kv_heads, block, 128))

@@ -355,7 +355,7 @@ class CudaOps(MixerOps, HybridOps, Fp8Ops):
         if not isinstance(k_cache, Fp8KVCache):
             return True
         _, kv_heads, block_size, _ = k_cache.shape
-        return self.decode_attention_mode != "flat" and bool(self.C.decode_fp8_qkv_pays(batch.padded_seqs, num_heads, kv_heads, block_size, batch.table_width))
+        return self.decode_attention_mode != "flat" and self.C.decode_fp8_qkv_pays(batch.padded_seqs, num_heads, kv_heads, block_size, batch.table_width)
 
     def decode_attention_qkv(self, qkv, q_weight, k_weight, eps, table, k_cache, v_cache, batch, num_heads, scale, do_rope=True):
         """Decode step: attention straight from the raw qkv projection.  q/k-norm, rotation at position len - 1 and the
