@@ -233,55 +233,61 @@ extern "C" int forge_fp8_store(const void* qkv, long long ld, const void* qw, co
 // ---------------------------------------------------------------------------------------------------------
 // Pages of sequences, in order, as bf16.  A CTA takes `rows` token rows of one page of one head of K or V.  Lengths, table entry and, once the
 // latter is there, the codes are asked for one after the other; where the page goes is found out meanwhile.  Bound by memory.
+// A CTA may be there while the kernel before still writes the cache, so nothing that is read here may pass for constant over the kernel's life
+// (no __restrict__): the loads stay behind the wait.
 // ---------------------------------------------------------------------------------------------------------
 constexpr int kExpandThreads = 128, kExpandLoads = 8;           // 28 x 100 .. 1024 in pages of 256 / of 64: 256 threads 19.6 / 25.3 us, 128 17.9 / 16.3, 64 18.6 / 17.4
 
-__global__ void __launch_bounds__(kExpandThreads) fp8_expand_kernel(
-    const uint8_t* __restrict__ k_codes, const uint8_t* __restrict__ k_scales, const uint8_t* __restrict__ v_codes,
-    const uint8_t* __restrict__ v_scales, const int* __restrict__ block_tables, const int* __restrict__ lens, int table_width, int num_blocks,
-    int nkv, int block_size, int rows, __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out, int* __restrict__ tables,
-    int capacity, unsigned* status) {
+struct Fp8Expand {
+  const uint8_t *k_codes, *k_scales, *v_codes, *v_scales;
+  const int *block_tables, *lens;
+  int table_width, num_blocks, nkv, block_size;
+  int rows;                                             // of a CTA: at most kExpandLoads * kExpandThreads / 16
+  __nv_bfloat16 *k_out, *v_out;
+  int* tables;
+  int capacity;
+  unsigned* status;
+};
+
+__global__ void __launch_bounds__(kExpandThreads) fp8_expand_kernel(const Fp8Expand a) {
   __shared__ int red[kExpandThreads / 32];
-  const int seq = blockIdx.y, page = blockIdx.x;
+  const int seq = blockIdx.y, page = blockIdx.x, block_size = a.block_size, rows = a.rows;
   const int parts = block_size / rows, z = blockIdx.z;
-  const int part = z % parts, kvh = z / parts % nkv, is_v = z / parts / nkv;
-  const int cap = table_width * block_size;
+  const int part = z % parts, kvh = z / parts % a.nkv, is_v = z / parts / a.nkv;
+  const int cap = a.table_width * block_size;
   const bool scribe = z == 0 && threadIdx.x == 0;       // writes the page's table entry
   pdl_launch_dependents();
   pdl_wait();
-  int len = lens[seq];
-  int blk = block_tables[static_cast<size_t>(seq) * table_width + page];
+  int len = a.lens[seq];
+  int blk = a.block_tables[static_cast<size_t>(seq) * a.table_width + page];
   int before = 0;                                       // pages of the sequences before this one
-  for (int i = threadIdx.x; i < seq; i += kExpandThreads) before += (min(max(lens[i], 0), cap) + block_size - 1) / block_size;
+  for (int i = threadIdx.x; i < seq; i += kExpandThreads) before += (min(max(a.lens[i], 0), cap) + block_size - 1) / block_size;
   if (len > cap) {
-    if (scribe && page == 0) set_status(status, kStatusBadIndex);
+    if (scribe && page == 0) set_status(a.status, kStatusBadIndex);
     len = cap;
   }
-  int* entry = tables + static_cast<size_t>(seq) * table_width + page;
+  int* entry = a.tables + static_cast<size_t>(seq) * a.table_width + page;
   if (page * block_size >= len) {
     if (scribe) *entry = -1;
     return;
   }
-  if (blk < 0 || blk >= num_blocks) {
-    if (scribe) set_status(status, kStatusBadIndex);
+  if (blk < 0 || blk >= a.num_blocks) {
+    if (scribe) set_status(a.status, kStatusBadIndex);
     blk = 0;
   }
-  const size_t row0 = (static_cast<size_t>(blk) * nkv + kvh) * block_size + part * rows;
+  const size_t row0 = (static_cast<size_t>(blk) * a.nkv + kvh) * block_size + part * rows;
   const int live = min(len - page * block_size - part * rows, rows);
-  const uint8_t* codes = (is_v ? v_codes : k_codes) + row0 * kFp8D;
-  const uint8_t* scales = (is_v ? v_scales : k_scales) + row0;
-  uint2 raw[kExpandLoads];
+  const uint8_t* codes = (is_v ? a.v_codes : a.k_codes) + row0 * kFp8D;
+  const uint8_t* scales = (is_v ? a.v_scales : a.k_scales) + row0;
+  uint2 raw[kExpandLoads];                              // 8 codes each; zeros behind the last token
   uint32_t scale[kExpandLoads];
-  const auto fetch = [&](int i0) {                      // 8 codes each; zeros behind the last token
 #pragma unroll
-    for (int k = 0; k < kExpandLoads; ++k) {
-      const int i = i0 + k * kExpandThreads;
-      const bool in = i >> 4 < live;
-      raw[k] = in ? *reinterpret_cast<const uint2*>(codes + static_cast<size_t>(i) * 8) : make_uint2(0, 0);
-      scale[k] = in ? scales[i >> 4] : 0u;
-    }
-  };
-  fetch(threadIdx.x);
+  for (int k = 0; k < kExpandLoads; ++k) {
+    const int i = threadIdx.x + k * kExpandThreads;
+    const bool in = i >> 4 < live;
+    raw[k] = in ? *reinterpret_cast<const uint2*>(codes + static_cast<size_t>(i) * 8) : make_uint2(0, 0);
+    scale[k] = in ? scales[i >> 4] : 0u;
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = before;
@@ -290,26 +296,23 @@ __global__ void __launch_bounds__(kExpandThreads) fp8_expand_kernel(
 #pragma unroll
   for (int i = 0; i < kExpandThreads / 32; ++i) before += red[i];
   const int to = before + page;
-  if (to >= capacity) {
+  if (to >= a.capacity) {
     if (scribe) {
-      set_status(status, kStatusBadIndex);
+      set_status(a.status, kStatusBadIndex);
       *entry = -1;
     }
     return;
   }
   if (scribe) *entry = to;
-  __nv_bfloat16* out = (is_v ? v_out : k_out) + ((static_cast<size_t>(to) * nkv + kvh) * block_size + part * rows) * kFp8D;
-  for (int i0 = threadIdx.x; i0 < rows * 16; i0 += kExpandLoads * kExpandThreads) {
-    if (i0 != threadIdx.x) fetch(i0);
+  __nv_bfloat16* out = (is_v ? a.v_out : a.k_out) + ((static_cast<size_t>(to) * a.nkv + kvh) * block_size + part * rows) * kFp8D;
 #pragma unroll
-    for (int k = 0; k < kExpandLoads; ++k) {
-      const int i = i0 + k * kExpandThreads;
-      if (i >= rows * 16) break;
-      const float m = fp8_scale(scale[k]);
-      const float2 f0 = fp8_to_float2(raw[k].x), f1 = fp8_to_float2(raw[k].x >> 16), f2 = fp8_to_float2(raw[k].y), f3 = fp8_to_float2(raw[k].y >> 16);
-      *reinterpret_cast<uint4*>(out + static_cast<size_t>(i) * 8) =
-          make_uint4(pack_bf16x2(f0.x * m, f0.y * m), pack_bf16x2(f1.x * m, f1.y * m), pack_bf16x2(f2.x * m, f2.y * m), pack_bf16x2(f3.x * m, f3.y * m));
-    }
+  for (int k = 0; k < kExpandLoads; ++k) {
+    const int i = threadIdx.x + k * kExpandThreads;
+    if (i >= rows * 16) break;
+    const float m = fp8_scale(scale[k]);
+    const float2 f0 = fp8_to_float2(raw[k].x), f1 = fp8_to_float2(raw[k].x >> 16), f2 = fp8_to_float2(raw[k].y), f3 = fp8_to_float2(raw[k].y >> 16);
+    *reinterpret_cast<uint4*>(out + static_cast<size_t>(i) * 8) =
+        make_uint4(pack_bf16x2(f0.x * m, f0.y * m), pack_bf16x2(f1.x * m, f1.y * m), pack_bf16x2(f2.x * m, f2.y * m), pack_bf16x2(f3.x * m, f3.y * m));
   }
 }
 
@@ -326,10 +329,10 @@ extern "C" int forge_fp8_expand(const void* k_codes, const void* k_scales, const
   const long long z = 2ll * nkv * (block_size / rows);
   if (z > 65535) return -1;
   const dim3 grid(static_cast<unsigned>(table_width), static_cast<unsigned>(num_seqs), static_cast<unsigned>(z));
-  return launch_kernel(fp8_expand_kernel, grid, dim3(kExpandThreads), 0, stream, 0, static_cast<const uint8_t*>(k_codes),
-                       static_cast<const uint8_t*>(k_scales), static_cast<const uint8_t*>(v_codes), static_cast<const uint8_t*>(v_scales), block_tables,
-                       lens, table_width, num_blocks, nkv, block_size, rows, static_cast<__nv_bfloat16*>(k_out), static_cast<__nv_bfloat16*>(v_out),
-                       tables, capacity, status) == cudaSuccess ? 0 : -2;
+  const Fp8Expand a{static_cast<const uint8_t*>(k_codes), static_cast<const uint8_t*>(k_scales), static_cast<const uint8_t*>(v_codes),
+                    static_cast<const uint8_t*>(v_scales), block_tables, lens, table_width, num_blocks, nkv, block_size, rows,
+                    static_cast<__nv_bfloat16*>(k_out), static_cast<__nv_bfloat16*>(v_out), tables, capacity, status};
+  return launch_kernel(fp8_expand_kernel, grid, dim3(kExpandThreads), 0, stream, 0, a) == cudaSuccess ? 0 : -2;
 }
 
 }  // namespace forge

@@ -1,5 +1,7 @@
 """Keys, values and normed rows in 8 bits on the PyTorch op set: formats, refusals, ops against 64 bits, the engine."""
+import pathlib
 import random
+import re
 import types
 import weakref
 
@@ -305,3 +307,12 @@ def test_the_rule_for_steps_from_the_raw_projection_refuses_heads_that_do_not_go
     for heads, kv_heads, block in ((4, 8, 64), (0, 1, 64), (7, 2, 64), (4, 0, 64), (-8, 8, 64), (8, 8, 24), (8, 8, 8)):
         with pytest.raises(RuntimeError, match="decode_fp8_qkv_pays"):
             ops.decodes_from_projection(step, heads, Fp8KVCache.zeros(2, kv_heads, block, 128))
+
+
+@pytest.mark.parametrize("source", ["attn/fp8_cache.cu", "attn/decode_fp8.cu", "elt/norm_fp8.cu", "include/fp8_cache.cuh"])
+def test_kernels_take_nothing_for_constant_that_the_kernel_before_them_writes(source):
+    """They start beside their predecessor's end, and a pointer to const that is declared restrict lets the compiler load through it before the
+    wait, or through a cache that is not kept up to date."""
+    text = (pathlib.Path(__file__).parent.parent / "csrc" / source).read_text()
+    code = re.sub(r"//[^\n]*", "", text)
+    assert "__restrict__" not in code and "__ldg" not in code and "ld.global.nc" not in code

@@ -235,6 +235,29 @@ def test_expand_leaves_out_what_does_not_fit_and_reports_it(ops):
     ops.status.zero_()
 
 
+def test_pages_are_read_back_as_the_store_before_left_them(ops):
+    """Store and read back in turn, without a pause: every time the values just written."""
+    lens, bs, nkv = [300, 77, 513], 64, 2
+    _, kc, vc, step = _paged(lens, nkv, nkv, bs)
+    gen, pages = _gen(8), sum(-(-n // bs) for n in lens)
+    slots = torch.cat([step.block_tables[i, torch.arange(n, device="cuda") // bs] * bs + torch.arange(n, device="cuda") % bs for i, n in enumerate(lens)]).int()
+    table, kept = ref.rope_table(8, 128, 1e4, "cuda"), []
+    projections = [_randn(gen, sum(lens), 3 * nkv * 128).to(BF) for _ in range(20)]
+    torch.cuda.synchronize()
+    for qkv in projections:
+        ops.qk_norm_rope_store(qkv, None, None, 1e-6, table, slots % 8, slots, kc, vc, nkv, nkv, 128, do_rope=False)
+        kept.append(ops.expand_kv(kc, vc, step.block_tables, step.context_lens, pages))
+    for qkv, (k, v, tables) in zip(projections, kept):
+        heads = qkv.view(-1, 3 * nkv, 128)
+        for got, x in ((k, heads[:, nkv:2 * nkv]), (v, heads[:, 2 * nkv:])):
+            want = Fp8KVCache(*quantize_heads(x.float())).dequantize().to(BF)
+            at = 0
+            for i, n in enumerate(lens):
+                assert torch.equal(got[tables[i, :-(-n // bs)].long()].transpose(1, 2).reshape(-1, nkv, 128)[:n], want[at:at + n])
+                at += n
+    ops.check_status()
+
+
 def test_every_code_and_scale_reads_back_exactly(ops):
     codes = torch.arange(256, device="cuda", dtype=torch.uint8).view(2, 128)
     scales = torch.arange(256, device="cuda", dtype=torch.uint8)
