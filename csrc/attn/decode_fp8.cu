@@ -151,7 +151,7 @@ struct F8Ring {
   static constexpr int kTile = 32 * kWarps, kHalf = kTile * kFp8D, kBytes = kStages * (2 * kHalf + 2 * kTile);
   uint8_t *codes, *scales;                             // [stage][K, V][tokens][128], [stage][K, V][tokens]
   uint64_t *full, *empty;
-  int s = 0, phase = 0;
+  int s = 0, phase = 0, issued = 0;                    // issued: tiles that may be on their way, at most kStages
   __device__ __forceinline__ void next() {
     if (++s == kStages) {
       s = 0;
@@ -198,9 +198,22 @@ struct F8Ring {
         bulk_load(sc + kTile, a.v_scales + row, rows, &full[s]);
       }
       __syncwarp();
+      issued = min(issued + 1, kStages);
       next();
     }
     return true;
+  }
+  // By the loading warp, at its end: waits for the last copies, so that none is on its way to the shared memory of a CTA that has left because a wait
+  // had run out.  (Otherwise the consumers wait for them.)
+  __device__ __forceinline__ void settle(unsigned* status, int lane) {
+    if (lane == 0) {
+      bool ok = true;
+      for (int i = 1; i <= issued && ok; ++i) {
+        const int at = s - i;
+        ok = mbar_wait_parked(&full[at < 0 ? at + kStages : at], at < 0 ? phase ^ 1 : phase, status);
+      }
+    }
+    __syncwarp();
   }
   static __device__ __forceinline__ int entry(const Fp8Decode& a, int seq, int page) {
     return page < a.table_width ? a.block_tables[static_cast<size_t>(seq) * a.table_width + page] : -1;
@@ -536,7 +549,7 @@ decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
 
   // the items of this share, in order; every role walks the same list
   int seq = start.seq, item = start.item, n = start.n, j = start.j, base = start.base;
-  bool ok = true;                                      // once a wait has run out none is made any more, but every barrier still is
+  bool ok = true;                                      // once a wait has run out none is made any more and no stage given back, but every barrier still is
   F8State st;
   while (base + kF8ItemCost + j < u_end) {
     const int count = min(n - j, u_end - (base + kF8ItemCost + j)), len = min(a.lens[seq], cap);
@@ -555,7 +568,7 @@ decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           st.take(K, K + F8FlatRing::kHalf, sc, sc + F8FlatRing::kTile, valid, lane);
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&ring.empty[ring.s]);
+        if (ok && lane == 0) mbar_arrive(&ring.empty[ring.s]);
       }
       st.sum_up();
       if (warp > 0) st.publish(s_join + (warp - 1) * F8State::kJoinFloats, s_join + (warp - 1) * F8State::kJoinFloats + F8State::kOFloats, lane);
@@ -586,6 +599,7 @@ decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       n = s_before[seq + 1] - s_before[seq] - kF8ItemCost;
     }
   }
+  if (warp == kF8Warps) ring.settle(a.status, lane);
 }
 
 // Joins the parts of an item that was cut.  A CTA for a cut and a head, its warps take the parts in turn.  Four warps with 32 registers find place beside
@@ -689,6 +703,7 @@ decode_fp8_cluster_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid
   const int n = (len + F8ClusterRing::kTile - 1) / F8ClusterRing::kTile, j = n * rank / C, count = n * (rank + 1) / C - j;
   if (warp == kF8CWarps) {
     ring.load(a, &tm_k, &tm_v, seq, kvh, len, j, count, 0, held, lane);
+    ring.settle(a.status, lane);
   } else {
     F8State st;
     if constexpr (kRaw) {
@@ -711,7 +726,7 @@ decode_fp8_cluster_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid
         st.take(K, K + F8ClusterRing::kHalf, sc, sc + F8ClusterRing::kTile, valid, lane);
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&ring.empty[ring.s]);
+      if (ok && lane == 0) mbar_arrive(&ring.empty[ring.s]);
     }
     st.sum_up();
     // what a warp has takes the place of its own rows of the first stage, which no other reads and into which nothing is loaded any more

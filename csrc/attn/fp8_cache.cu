@@ -134,6 +134,7 @@ __global__ void __launch_bounds__(32 * (kStoreWarps + 1), kStoreCtasPerSm) fp8_s
   };
   if (warp == consumers) {
     bool ok = true;
+    int issued = 0;                                      // rows that may be on their way, at most as many as there are stages
     for (int t0 = blockIdx.x; t0 < a.T && ok; t0 += 32 * gridDim.x) {             // slots and positions of 32 tokens at a time
       const int mine = t0 + lane * gridDim.x;
       const int slot = mine < a.T ? a.slots[mine] : -1, at = mine < a.T && a.rope != nullptr ? fp8_angle_row(a, a.positions[mine]) : 0;
@@ -152,8 +153,15 @@ __global__ void __launch_bounds__(32 * (kStoreWarps + 1), kStoreCtasPerSm) fp8_s
           }
         }
         ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (!ok) break;
+        issued = min(issued + 1, stages);
         next();
       }
+    }
+    // none may be on its way to a CTA that has left because a wait had run out
+    for (int i = 1; i <= issued && lane == 0; ++i) {
+      const int at = s - i;
+      if (!mbar_wait_parked(&full[at < 0 ? at + stages : at], at < 0 ? phase ^ 1 : phase, a.status)) break;
     }
     return;
   }
