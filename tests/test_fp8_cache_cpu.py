@@ -316,3 +316,31 @@ def test_kernels_take_nothing_for_constant_that_the_kernel_before_them_writes(so
     text = (pathlib.Path(__file__).parent.parent / "csrc" / source).read_text()
     code = re.sub(r"//[^\n]*", "", text)
     assert "__restrict__" not in code and "__ldg" not in code and "ld.global.nc" not in code
+
+
+@pytest.mark.parametrize("ahead", [0, 1, 3])
+def test_decode_steps_built_one_after_the_other_equal_rebuilt_ones(ahead):
+    """Tables that grow as sequences do, with blocks reserved ahead at any time: equal in every word, but for entries behind the newest token's block."""
+    from tinyllmforge_b200.engine.request import Request
+    from tinyllmforge_b200.engine.step_batch import DecodeBuilder, build_decode
+    rng, bs, width = random.Random(ahead), 8, 16
+    reqs = [Request(list(range(n)), SamplingParams(temperature=0.5)) for n in (1, 7, 8, 9, 30)]
+    free = iter(range(1000))
+    builder = DecodeBuilder(bs)
+    for step in range(60):
+        for r in reqs:
+            need = -(-len(r) // bs) + (rng.randint(0, ahead) if rng.random() < 0.3 else 0)
+            r.block_table += [next(free) for _ in range(need - len(r.block_table))]
+        got, want = builder.build(reqs, step, 5, 8, width), build_decode(reqs, bs, step, 5, 8, width)
+        a, b = got.buf[:got.num_words].copy(), want.buf
+        at, size = got.offsets["block_tables"]
+        for i, r in enumerate(reqs):
+            last = (len(r) - 1) // bs + 1                # entries that are read
+            rows = [x[at + i * width:at + (i + 1) * width] for x in (a, b)]
+            assert rows[0][:last].tolist() == rows[1][:last].tolist() == r.block_table[:last]
+            for x in rows:
+                if ahead:
+                    x[last:] = -1
+        assert (a == b).all()
+        for r in reqs:
+            r.append_token(rng.randrange(100))

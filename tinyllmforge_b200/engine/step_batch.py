@@ -230,7 +230,8 @@ class DecodeBuilder:
     only by: every length + 1, the new input token of every request, and an occasional new block id.  The packed
     buffer of the previous step is updated in place with a few vector operations instead of being rebuilt from
     the request objects (the reference rebuilds five Python lists over all sequences every step,
-    tinyvllm/engine/model_runner.py:210-228).  Produces exactly what ``build_decode`` produces.
+    tinyvllm/engine/model_runner.py:210-228).  Produces what ``build_decode`` produces, but for table entries behind the block of a
+    sequence's newest token, which nothing reads: blocks that were reserved further ahead are copied when the sequence reaches them.
     """
 
     def __init__(self, block_size: int):
