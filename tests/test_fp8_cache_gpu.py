@@ -886,6 +886,87 @@ def test_model_in_8_bits_is_as_near_to_the_full_one_as_the_fp32_ops_are(quantiza
     ops.check_status()
 
 
+def _requests(cfg, lens):
+    from tinyllmforge_b200 import SamplingParams
+    from tinyllmforge_b200.engine.request import Request
+    rng, reqs = np.random.default_rng(1), []
+    for i, n in enumerate(lens):
+        r = Request(rng.integers(0, cfg.vocab_size, n).tolist(), SamplingParams(temperature=0.0))
+        r.block_table = [2 * i, 2 * i + 1]
+        reqs.append(r)
+    return reqs
+
+
+def _batch(sb):
+    from tinyllmforge_b200.engine.worker import DeviceBatch
+    return DeviceBatch(sb, torch.from_numpy(sb.buf[:sb.num_words].copy()).cuda())
+
+
+@pytest.mark.parametrize("quantization", [None, "fp8_block"])
+def test_a_models_decode_step_has_the_same_bits_with_one_op_and_with_two(quantization, monkeypatch):
+    """Attention from the raw projection against store and attention: hidden states and caches of every layer, step after step."""
+    from tinyllmforge_b200.engine.step_batch import build_decode, build_prefill
+    cfg, _, _, gpu, ops = _models(quantization)
+    monkeypatch.setattr(ops, "decode_attention_mode", "chunked")
+    one, rng, calls = gpu.kv_cache, np.random.default_rng(2), []
+    fused = ops.decode_attention_qkv_fp8
+    monkeypatch.setattr(ops, "decode_attention_qkv_fp8", lambda *a: calls.append(1) or fused(*a))
+    reqs = _requests(cfg, (5, 300, 257))
+    with torch.inference_mode():
+        gpu.forward(_batch(build_prefill(reqs, 256)))
+        two = _copy(one)[0]
+        for _ in range(3):
+            for r in reqs:
+                r.append_token(int(rng.integers(0, cfg.vocab_size)))
+            batch, hidden = _batch(build_decode(reqs, 256)), []
+            for cache, most in ((one, 32), (two, 0)):
+                monkeypatch.setattr(ops, "fused_qkv_max_batch", most)
+                gpu.bind_kv_cache(cache)
+                hidden.append(gpu.forward(batch).clone())
+                assert len(calls) == (3 if most else 0)              # layers
+                calls.clear()
+            assert torch.equal(*hidden) and _same_cache(one, two) and hidden[0].isfinite().all()
+    ops.check_status()
+
+
+def test_the_block_loop_with_8_bit_rows_is_its_ops_one_after_the_other(monkeypatch):
+    """A prompt step and decode steps of the whole model against the ops by hand, with the residual stream added up in plain PyTorch: equal bits."""
+    from tinyllmforge_b200.engine.step_batch import build_decode, build_prefill
+    cfg, _, _, gpu, ops = _models("fp8_block")
+    mine = gpu.kv_cache
+    other = _copy(mine)[0]
+    norms, rng = [], np.random.default_rng(3)
+    norm = ops.rms_norm_fp8
+    monkeypatch.setattr(ops, "rms_norm_fp8", lambda *a: norms.append(1) or norm(*a))
+
+    def by_hand(batch):
+        stream = gpu.embed_tokens.weight[batch.input_ids.long()]
+        rows = lambda s, w: norm(s.clone(), None, w, cfg.rms_norm_eps)[0]
+        for i, l in enumerate(gpu.layers):
+            qkv = ops.linear(rows(stream, l.input_layernorm), l.qkv_proj.weight)
+            q = ops.qk_norm_rope_store(qkv, l.q_norm, l.k_norm, cfg.rms_norm_eps, gpu.rope, batch.positions, batch.slot_mapping, other[i, 0], other[i, 1],
+                                       cfg.num_attention_heads, cfg.num_key_value_heads, 128)
+            a = ops.attention(q, other[i, 0], other[i, 1], batch, SCALE)
+            stream = (stream.float() + ops.linear(a, l.o_proj.weight).float()).to(BF)
+            y = ops.linear(rows(stream, l.post_attention_layernorm), l.gate_up_proj.weight)
+            x = ops.linear(ops.silu_mul(y), l.down_proj.weight)
+            if i + 1 < len(gpu.layers):
+                stream = (stream.float() + x.float()).to(BF)
+        return ops.add_rms_norm(x, stream.clone(), gpu.norm, cfg.rms_norm_eps)[0]
+
+    reqs = _requests(cfg, (5, 70, 40))
+    with torch.inference_mode():
+        for step in range(4):
+            batch = _batch(build_prefill(reqs, 256) if step == 0 else build_decode(reqs, 256))
+            got, want = gpu.forward(batch), by_hand(batch)
+            assert len(norms) == 2 * len(gpu.layers)     # the loop with 8-bit rows
+            norms.clear()
+            assert torch.equal(got, want) and got.isfinite().all() and _same_cache(mine, other)
+            for r in reqs:
+                r.append_token(int(rng.integers(0, cfg.vocab_size)))
+    ops.check_status()
+
+
 @pytest.mark.parametrize("quantization", [None, "fp8_block"])
 def test_engine_loops_graphs_chunks_and_prefix_cache_agree_with_an_8_bit_cache(quantization):
     from tinyllmforge_b200 import LLM, SamplingParams, preset
