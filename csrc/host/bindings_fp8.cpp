@@ -126,6 +126,9 @@ std::tuple<Tensor, Tensor, Tensor> fp8_expand(const Tensor& k_codes, const Tenso
   return {k_out, v_out, tables};
 }
 
+// The attention kernels round lengths up to whole tiles of up to 128 tokens in 32 bits.
+constexpr int64_t kMostTokens = INT32_MAX - 127;
+
 // Returns [sequences, nq * 128].  mode: 0 by size, 1 equal shares over the GPU, 2 a cluster of CTAs per sequence and KV head.
 Tensor decode_fp8(const Tensor& q, const Tensor& k_codes, const Tensor& k_scales, const Tensor& v_codes, const Tensor& v_scales,
                   const Tensor& block_tables, const Tensor& lens, double scale, const Tensor& status, int64_t mode) {
@@ -135,7 +138,7 @@ Tensor decode_fp8(const Tensor& q, const Tensor& k_codes, const Tensor& k_scales
   const int64_t B = q.size(0), nq = q.size(1), W = block_tables.size(1);
   TORCH_CHECK(nq >= 1 && nq % k.nkv == 0, "decode_fp8: query heads must be a multiple of the KV heads");
   TORCH_CHECK(block_tables.size(0) >= B, "decode_fp8: a table for every sequence expected");
-  TORCH_CHECK(W * k.block <= INT32_MAX, "decode_fp8: too wide a table");
+  TORCH_CHECK(W * k.block <= kMostTokens, "decode_fp8: too wide a table");
   for (const Tensor* t : {&block_tables, &lens, &status}) same_device(*t, q, "decode_fp8");
   const void* qp = data(q, BF, 0, "decode_fp8: q");
   if (B > 0) aligned16(q, "decode_fp8: q");
@@ -163,7 +166,7 @@ Tensor decode_fp8_qkv(const Tensor& qkv, const OptTensor& qw, const OptTensor& k
   TORCH_CHECK(nq >= 1 && nq % k.nkv == 0, "decode_fp8_qkv: query heads must be a multiple of the KV heads");
   view2(qkv, BF, B, (nq + 2 * k.nkv) * 128, "decode_fp8_qkv: qkv");
   TORCH_CHECK(ld >= qkv.size(1) && ld % 8 == 0, "decode_fp8_qkv: rows of qkv overlap, or are not aligned to 16 bytes");
-  TORCH_CHECK(block_tables.size(0) >= B && W * k.block <= INT32_MAX, "decode_fp8_qkv: a table for every sequence expected, not too wide");
+  TORCH_CHECK(block_tables.size(0) >= B && W * k.block <= kMostTokens, "decode_fp8_qkv: a table for every sequence expected, not too wide");
   for (const Tensor* t : {&block_tables, &lens, &status}) same_device(*t, qkv, "decode_fp8_qkv");
   if (B > 0) aligned16(qkv, "decode_fp8_qkv: qkv");
   for (const OptTensor* w : {&qw, &kw})

@@ -722,6 +722,25 @@ def test_refusals(ops):
     ops.check_status()
 
 
+def test_tables_whose_lengths_do_not_round_up_in_32_bits_are_refused(ops):
+    """2^31 - 16 tokens, which a length that is too large is clamped to, are 2^31 in whole tiles."""
+    qkv, w, kc, vc, step, at, slots = _raw_case([40], 2, 1, 16)
+    tables = torch.zeros(1, 2 ** 27 - 1, dtype=I32, device="cuda")
+    wide = Step(is_prefill=False, block_tables=tables, context_lens=step.context_lens, table_width=tables.shape[1], padded_seqs=1, max_seqlen_k=40)
+    with pytest.raises(RuntimeError, match="wide"):
+        ops.attention(torch.zeros(1, 2, 128, dtype=BF, device="cuda"), kc, vc, wide, SCALE)
+    with pytest.raises(RuntimeError, match="wide"):
+        ops.decode_attention_qkv(qkv, *w, 1e-6, ref.rope_table(64, 128, 1e4, "cuda"), kc, vc, wide, 2, SCALE)
+    wide.block_tables = tables[:, :2 ** 27 - 8].contiguous()        # 2^31 - 128 tokens
+    wide.block_tables[0, :3] = step.block_tables[0, :3]
+    wide.table_width = wide.block_tables.shape[1]
+    got = ops.decode_attention_qkv(qkv, *w, 1e-6, ref.rope_table(64, 128, 1e4, "cuda"), kc, vc, wide, 2, SCALE)
+    q = ops.qk_norm_rope_store(qkv, *w, 1e-6, ref.rope_table(64, 128, 1e4, "cuda"), at, slots, kc, vc, 2, 1, 128)
+    _check_decode(got, q, kc, vc, step, [40])
+    _check_decode(ops.attention(q, kc, vc, wide, SCALE), q, kc, vc, step, [40])
+    ops.check_status()
+
+
 # ----------------------------------------------------------------------------- streams, graphs, order
 @pytest.mark.parametrize("mode", ["flat", "chunked"])
 def test_decode_gives_the_same_bits_again_and_on_another_stream(ops, mode, monkeypatch):
