@@ -418,6 +418,37 @@ def test_calls_without_tokens(ops):
     assert ops.expand_kv(kc, vc, none.block_tables, none.context_lens, 0)[0].shape == (0, 2, 16, 128)
 
 
+@pytest.mark.parametrize("nq,nkv", [(8, 2), (2, 1), (16, 2), (5, 1), (10, 1)])
+@pytest.mark.parametrize("mode", ["flat", "chunked"])
+def test_decode_with_whole_weights(ops, nq, nkv, mode, monkeypatch):
+    """Pairs of tokens with nearly the same key and opposite values: what is left of a pair is the difference of two weights, and a weight rounded to
+    a few bits shows.
+
+    Allowed: half a step of bf16 of the result, and of the mean |value|: twice (weight, and sum of the weights) 2^-19 for a weight (its exponent, up to 16,
+    is rounded twice, half a step of 2^-20 times ln 2 each, the power is within 2^-22, its two halves within 2^-22: 1.2 2^-20), 2^-20 of the score's
+    products (as in the oracle), and a step of 2^-23 for every token that is added up."""
+    monkeypatch.setattr(ops, "decode_attention_mode", mode)
+    lens = [2, 20, 34, 64, 130]
+    q, kc, vc, step = _paged(lens, nq, nkv, 64, spread=0.0, q_scale=0.1)
+    for i, n in enumerate(lens):
+        t = torch.arange(0, n, 2, device="cuda")
+        for c in (kc, vc):
+            b = step.block_tables[i, t // 64].long()
+            c.code_bytes[b, :, t % 64 + 1] = c.code_bytes[b, :, t % 64] ^ (0x80 if c is vc else 0)
+            c.scales[b, :, t % 64 + 1] = c.scales[b, :, t % 64]
+        kc.code_bytes[step.block_tables[i, t // 64].long(), :, t % 64 + 1, 5] &= 0xF8   # a key's entry moves by less than half, and stays a number
+    got = ops.attention(q, kc, vc, step, SCALE).to(F64).view(len(lens), nq, 128)
+    for i, n in enumerate(lens):
+        k, v = (oracle.sequence(c, step.block_tables[i], n).repeat_interleave(nq // nkv, 0) for c in (kc, vc))
+        p = torch.softmax(torch.einsum("hd,hnd->hn", q[i].to(F64), k) * SCALE, -1)
+        want, spread = torch.einsum("hn,hnd->hd", p, v), torch.einsum("hn,hnd->hd", p, v.abs())
+        size = (torch.einsum("hd,hnd->hn", q[i].to(F64).abs(), k.abs()) * SCALE).amax(-1, keepdim=True)
+        allowed = want.abs() * 2.0 ** -8 + spread * (2 * (2.0 ** -19 + 2.0 ** -20 * size) + n * 2.0 ** -23)
+        worst = ((got[i] - want).abs() / allowed).amax()
+        assert worst <= 1, f"sequence {i} of {n} tokens: {float(worst):.3g} times what is allowed"
+    ops.check_status()
+
+
 @pytest.mark.parametrize("mode", ["flat", "chunked"])
 def test_decode_over_a_long_context_with_a_common_direction(ops, mode, monkeypatch):
     """200000 values of one sign: sums that lose a little at every step would be off by the same sign."""
