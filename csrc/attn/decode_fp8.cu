@@ -13,11 +13,12 @@
 // bank once, and converts them in place; V^T needs no transposing load, two tokens' bytes are interleaved instead.
 //   Queries are brought to [2^14, 2^15) by a power of two per head, which keeps every bit of their bf16 down to 2^-31 of the largest entry.
 //   A value's scale 2^e goes into its weight's exponent: w_j = 2^(c q.k_j + e_j - u + 7), u a maximum of its own: a value that counts is never lost
-//   beside one with a larger scale that does not.  A weight is two halves, its first 11 bits and what is left of it, and both are multiplied: within 2^-22
-//   of itself, or 2^-31 of the largest (fp16 has no smaller numbers).  With the first half alone results were off by 2^-12 of the mean |value|, where
-//   those over a bf16 cache are not: 256 x 100 .. 1500 tokens 78.2 us, 80.1 so; 13 x 200 .. 2000 14.5, 15.1; 9 x 9000 .. 32000 69.7, 70.6;
-//   1 x 3001 9.2, 9.4.  The sum of the p_j is kept in fp32.  m and u move only when they are exceeded by 8, so w_j <= 2^15 and products are
-//   rescaled rarely.
+//   beside one with a larger scale that does not.  A weight is two halves, its first 11 bits and what is left of it: within 2^-22 of itself, or 2^-31 of
+//   the largest (fp16 has no smaller numbers).  With the first half alone results were off by 2^-12 of the mean |value|, where those over a
+//   bf16 cache are not.  Of up to four heads columns 4 .. 7 are the same heads once more, with the second halves, and the columns are added up
+//   at the item's end; of more heads both halves are multiplied.  The first half alone / columns / both, 32 / 8 heads: 16 x 768 tokens 11.8 / 12.1 /
+//   12.6 us, 32 x 768 15.3 / 15.8 / 16.6, 256 x 100 .. 1500 77.1 / 77.2 / 79.2.  The sum of the p_j is kept in fp32.  m and u move only when they are
+//   exceeded by 8, so w_j <= 2^15 and products are rescaled rarely.
 // What is behind a sequence's last token never counts: its scores, weights and value bytes are replaced, whatever they are.
 //
 // The split, many items.  The tiles of 64 tokens of all items, in order, are dealt out to four teams per SM, of two consumer warps and a loading one with a
@@ -223,6 +224,8 @@ struct F8Ring {
 
 // A consumer warp's share of an item.  Lane l = 4 g + quad holds scores of tokens g + 8 i and heads 2 quad, 2 quad + 1, and of the results dims
 // 16 g .. 16 g + 15 of these heads.
+// kWide: of more than four heads.  Otherwise heads 4 .. 7 are heads 0 .. 3 again, and their results are what the second halves of the weights add.
+template <bool kWide>
 struct F8State {
   uint32_t qh[16];                                     // 32 consecutive entries of head g, from 32 quad on
   float qf[2];                                         // of heads 2 quad, 2 quad + 1: from products to scores in base 2
@@ -230,7 +233,7 @@ struct F8State {
   float o[8][4];                                       // [i][0], [i][1]: dim 16 g + 2 i of heads 2 quad, 2 quad + 1; [2], [3]: the dim after it
 
   __device__ __forceinline__ void begin(const __nv_bfloat16* q_rows, int heads, float scale_log2, int lane) {
-    const int g = lane >> 2, quad = lane & 3;
+    const int g = kWide ? lane >> 2 : (lane >> 2) & 3, quad = lane & 3;
     uint32_t w[16], top = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -338,8 +341,9 @@ struct F8State {
         l[1] += ex2_approx(x[i][1] - m[1]);
         const float w0 = ex2_approx(y[i][0] - u0), w1 = ex2_approx(y[i][1] - u1);
         const float h0 = __uint_as_float(__float_as_uint(w0) & 0xFFFFE000u), h1 = __uint_as_float(__float_as_uint(w1) & 0xFFFFE000u);     // 11 bits
-        p[k] = transpose8x8(f8_half2(h0, h1));
-        rest[k] = transpose8x8(f8_half2(w0 - h0, w1 - h1));
+        const uint32_t whole = f8_half2(h0, h1), left = f8_half2(w0 - h0, w1 - h1);
+        p[k] = transpose8x8(kWide || quad < 2 ? whole : left);
+        if constexpr (kWide) rest[k] = transpose8x8(left);
       }
       // ---- values: of 16 tokens 2 quad, 2 quad + 1 and eight further on, dims 16 g ..
       uint32_t w[4][4];
@@ -359,8 +363,10 @@ struct F8State {
           fp8x4_to_half2(__byte_perm(w[2][e], w[3][e], h ? 0x7362 : 0x5140), f[h][2], f[h][3]);
           mma16816_f16(o[2 * e + h], f[h], p[0], p[1]);
         }
+        if constexpr (kWide) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) mma16816_f16(o[2 * e + h], f[h], rest[0], rest[1]);
+          for (int h = 0; h < 2; ++h) mma16816_f16(o[2 * e + h], f[h], rest[0], rest[1]);
+        }
       }
     }
   }
@@ -402,6 +408,10 @@ struct F8State {
   }
   // o <- results.
   __device__ __forceinline__ void finish() {
+    if constexpr (!kWide) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) o[i >> 2][i & 3] += __shfl_xor_sync(0xffffffffu, o[i >> 2][i & 3], 2);
+    }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const float f = l[h] == 0.f ? 0.f : 1.f / l[h] * exp2f(u[h] - m[h] - kF8Top);        // (no score: zeros)
@@ -447,7 +457,7 @@ constexpr int kF8ItemCost = 2;                         // tiles (1, 3: 256 x 100
 constexpr int kF8Share = 4;                            // units to a team at least, or there are fewer teams at work (2, 8: 13 x 200 .. 2000 13.7, 16.7 us for 13.4)
 using F8FlatRing = F8Ring<kF8Warps, kF8Stages>;
 
-constexpr int kF8JoinArea = (kF8Warps - 1) * F8State::kJoinFloats;
+constexpr int kF8JoinArea = (kF8Warps - 1) * F8State<true>::kJoinFloats;
 constexpr int kF8FlatSmem = 1024 + kF8Teams * (F8FlatRing::kBytes + kF8JoinArea * 4 + 2 * kF8Stages * 8) + (kF8Seqs + 1 + kF8Threads / 32) * 4;
 static_assert(kF8FlatSmem <= 227 * 1024, "shared memory");
 
@@ -472,6 +482,7 @@ __device__ __forceinline__ F8Place f8_place(const int* before, int B, int items,
   return p;
 }
 
+template <bool kWide>
 __global__ void __launch_bounds__(kF8Threads, 1)
 decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Fp8Decode a) {
   extern __shared__ uint8_t smem_raw[];
@@ -555,7 +566,8 @@ decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   // the items of this share, in order; every role walks the same list
   int seq = start.seq, item = start.item, n = start.n, j = start.j, base = start.base;
   bool ok = true;                                      // once a wait has run out none is made any more and no stage given back, but every barrier still is
-  F8State st;
+  using State = F8State<kWide>;
+  State st;
   while (base + kF8ItemCost + j < u_end) {
     const int count = min(n - j, u_end - (base + kF8ItemCost + j)), len = min(a.lens[seq], cap);
     const int kvh = item / a.slices, slice = item - kvh * a.slices, head0 = kvh * a.group + slice * a.G, heads = min(a.G, a.group - slice * a.G);
@@ -576,12 +588,12 @@ decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         if (ok && lane == 0) mbar_arrive(&ring.empty[ring.s]);
       }
       st.sum_up();
-      if (warp > 0) st.publish(s_join + (warp - 1) * F8State::kJoinFloats, s_join + (warp - 1) * F8State::kJoinFloats + F8State::kOFloats, lane);
+      if (warp > 0) st.publish(s_join + (warp - 1) * State::kJoinFloats, s_join + (warp - 1) * State::kJoinFloats + State::kOFloats, lane);
       named_barrier_sync(1 + team, 32 * kF8Warps);
       if (warp == 0) {
 #pragma unroll
         for (int w = 1; w < kF8Warps; ++w)
-          st.join(s_join + (w - 1) * F8State::kJoinFloats, s_join + (w - 1) * F8State::kJoinFloats + F8State::kOFloats, lane);
+          st.join(s_join + (w - 1) * State::kJoinFloats, s_join + (w - 1) * State::kJoinFloats + State::kOFloats, lane);
       }
       named_barrier_sync(1 + team, 32 * kF8Warps);            // the joining area is the next item's
       if (warp == 0) {
@@ -671,7 +683,7 @@ constexpr int f8_cluster_smem(int G, int stages) {
 
 // Grid (CTAs of an item, items): CTA r of C takes tiles [n r / C, n (r + 1) / C) of its item's n, and its share of the results is what all
 // of them left in their shared memory, joined.
-template <bool kRaw>
+template <bool kRaw, bool kWide>
 __global__ void __launch_bounds__(kF8CThreads, kF8CCtasPerSm)
 decode_fp8_cluster_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Fp8Decode a) {
   extern __shared__ uint8_t smem_raw[];
@@ -710,7 +722,7 @@ decode_fp8_cluster_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid
     ring.load(a, &tm_k, &tm_v, seq, kvh, len, j, count, 0, held, lane);
     ring.settle(a.status, lane);
   } else {
-    F8State st;
+    F8State<kWide> st;
     if constexpr (kRaw) {
       __nv_bfloat16* s_q = reinterpret_cast<__nv_bfloat16*>(s_o);        // free until results are there, after the next barrier but one
       if (4 * warp < heads) f8_make_queries(a, seq, head0, heads, len, warp, s_q, lane);
@@ -830,13 +842,13 @@ static bool f8_maps(const Fp8Decode& a, int tile, CUtensorMap* tm_k, CUtensorMap
   return forge_make_tmap_2d(tm_k, a.k_codes, rows, kFp8D, kFp8D, box, 1) == 0 && forge_make_tmap_2d(tm_v, a.v_codes, rows, kFp8D, kFp8D, box, 1) == 0;
 }
 
-template <bool kRaw>
+template <bool kRaw, bool kWide>
 static int f8_launch_clusters(Fp8Decode a, int C, cudaStream_t stream) {
   a.stages = static_cast<long long>(a.table_width) * a.block_size <= static_cast<long long>(C) * F8ClusterRing::kTile ? 1 : kF8CStages;
   CUtensorMap tm_k, tm_v;
   if (!f8_maps(a, F8ClusterRing::kTile, &tm_k, &tm_v)) return -2;
-  FORGE_ENSURE_DYN_SMEM(decode_fp8_cluster_kernel<kRaw>, f8_cluster_smem(kF8Heads, kF8CStages));
-  return launch_kernel_cluster_x(decode_fp8_cluster_kernel<kRaw>, dim3(C, static_cast<unsigned>(a.B * a.nkv * a.slices)), dim3(kF8CThreads), f8_cluster_smem(a.G, a.stages),
+  FORGE_ENSURE_DYN_SMEM((decode_fp8_cluster_kernel<kRaw, kWide>), f8_cluster_smem(kF8Heads, kF8CStages));
+  return launch_kernel_cluster_x(decode_fp8_cluster_kernel<kRaw, kWide>, dim3(C, static_cast<unsigned>(a.B * a.nkv * a.slices)), dim3(kF8CThreads), f8_cluster_smem(a.G, a.stages),
                                  stream, C, tm_k, tm_v, a) == cudaSuccess ? 0 : -5;
 }
 
@@ -861,18 +873,21 @@ extern "C" int forge_decode_fp8(const void* q, const void* k_codes, const void* 
   Fp8Decode a = f8_operands(const_cast<void*>(k_codes), const_cast<void*>(k_scales), const_cast<void*>(v_codes), const_cast<void*>(v_scales), block_tables,
                             lens, out, z, B, nq, nkv, block_size, table_width, num_blocks, scale, status);
   a.q = static_cast<const __nv_bfloat16*>(q);
-  if (const int C = f8_cluster(static_cast<long long>(B) * nkv * z.slices, table_width, block_size, mode)) return f8_launch_clusters<false>(a, C, stream);
+  if (const int C = f8_cluster(static_cast<long long>(B) * nkv * z.slices, table_width, block_size, mode))
+    return z.G > 4 ? f8_launch_clusters<false, true>(a, C, stream) : f8_launch_clusters<false, false>(a, C, stream);
   const long long tiles = (static_cast<long long>(table_width) * block_size + F8FlatRing::kTile - 1) / F8FlatRing::kTile;
   if (std::min(B, kF8Seqs) * (tiles + kF8ItemCost) * nkv * z.slices > INT32_MAX) return -1;
   CUtensorMap tm_k, tm_v;
   if (!f8_maps(a, F8FlatRing::kTile, &tm_k, &tm_v)) return -2;
-  FORGE_ENSURE_DYN_SMEM(decode_fp8_kernel, kF8FlatSmem);
+  FORGE_ENSURE_DYN_SMEM(decode_fp8_kernel<true>, kF8FlatSmem);
+  FORGE_ENSURE_DYN_SMEM(decode_fp8_kernel<false>, kF8FlatSmem);
+  const auto shares = z.G > 4 ? decode_fp8_kernel<true> : decode_fp8_kernel<false>;
   a.cuts = reinterpret_cast<int4*>(scratch);
   a.part_o = scratch + 4ll * z.teams;
   a.part_ml = a.part_o + 2ll * z.teams * z.G * kFp8D;
   for (int left = B; left > 0; left -= kF8Seqs) {
     a.B = std::min(left, kF8Seqs);
-    if (launch_kernel(decode_fp8_kernel, dim3(z.ctas), dim3(kF8Threads), kF8FlatSmem, stream, 0, tm_k, tm_v, a) != cudaSuccess) return -5;
+    if (launch_kernel(shares, dim3(z.ctas), dim3(kF8Threads), kF8FlatSmem, stream, 0, tm_k, tm_v, a) != cudaSuccess) return -5;
     if (launch_kernel(decode_fp8_join_kernel, dim3(z.teams, z.G), dim3(a.B * nkv * z.slices <= 32 ? 256 : 128), 0, stream, 0, a) != cudaSuccess) return -5;
     a.q += static_cast<size_t>(kF8Seqs) * nq * kFp8D;
     a.block_tables += static_cast<size_t>(kF8Seqs) * table_width;
@@ -896,7 +911,7 @@ extern "C" int forge_decode_fp8_qkv(const void* qkv, long long ld, const void* q
   a.qkv = static_cast<const __nv_bfloat16*>(qkv); a.ld_qkv = ld;
   a.qw = static_cast<const __nv_bfloat16*>(qw); a.kw = static_cast<const __nv_bfloat16*>(kw);
   a.eps = eps; a.rope = rope; a.rope_rows = rope_rows;
-  return f8_launch_clusters<true>(a, C, stream);
+  return z.G > 4 ? f8_launch_clusters<true, true>(a, C, stream) : f8_launch_clusters<true, false>(a, C, stream);
 }
 
 }  // namespace forge
