@@ -805,9 +805,12 @@ static F8Grid f8_grid(int B, int nq, int nkv, int block_size, int table_width) {
   return z;
 }
 
-// CTAs of an item's cluster, 0: equal shares over the GPU.  mode 1: equal shares, 2: clusters, 0: by size, the longest context being as long as the
-// block table is wide.  Measured, equal shares / clusters, us, 32 / 8 heads.  Clusters of 8: 1 x 700 tokens 9.4 / 6.2, 1 x 6000 12.1 / 10.9, 1 x 9000
-// 12.7 / 13.7, 1 x 16000 14.5 / 21.7, 4 x 6000 15.6 / 13.2, 4 x 9000 17.6 / 17.5.  Of 4: 8 x 200 .. 2000 11.7 / 9.7, 8 x 3000 14.8 / 12.7, 8 x 5000
+// CTAs of an item's cluster, 0: equal shares over the GPU.  mode 1: equal shares, 2: clusters, 0: by size, the longest context being taken to be as
+// long as the block table is wide.  That is so where the caller cuts the table to the step; the engine's captured steps have tables of max_model_len
+// tokens, whatever the contexts, so with 8 KV heads they take clusters up to 8 sequences at 4096, up to 4 at 8192 and none beyond (16 x 768 tokens, 32 / 8
+// heads, in a table of 768 / 4096: 9.3 / 12.1 us; 1 x 1000 in one of 8192 / 32768: 6.0 / 10.1).
+// Measured with tables as wide as the longest context and weights of 11 bits (with 22 both are 1 to 3 % slower), equal shares / clusters, us, 32 / 8 heads.
+// Clusters of 8: 1 x 700 tokens 9.4 / 6.2, 1 x 6000 12.1 / 10.9, 1 x 9000 12.7 / 13.7, 1 x 16000 14.5 / 21.7, 4 x 6000 15.6 / 13.2, 4 x 9000 17.6 / 17.5.  Of 4: 8 x 200 .. 2000 11.7 / 9.7, 8 x 3000 14.8 / 12.7, 8 x 5000
 // 18.2 / 19.0.  Of 2, for which lengths that differ count more: 16 x 768 11.9 / 9.1, 16 x 1500 14.4 / 12.7, 16 x 200 .. 1500 12.2 / 12.0, 13 x 200 .. 2000
 // 12.2 / 14.2.  One CTA: 32 x 768 15.4 / 11.5, 32 x 100 .. 768 12.0 / 10.7, 32 x 100 .. 1024 13.4 / 13.2, 32 x 1500 21.9 / 22.4.  More than 256 CTAs: 100 x
 // 100 .. 300 16.8 / 18.0.  8 / 1 heads: 32 x 200 .. 2000 (clusters of 8) 13.8 / 7.5, 64 x 100 .. 500 12.2 / 6.3.  Clusters of 8 find no place beside

@@ -227,7 +227,7 @@ extern "C" int forge_fp8_store(const void* qkv, long long ld, const void* qw, co
   const int stages = std::min(kStoreMaxStages, kStoreSmem / stage);
   // Measured, a warp per set / ring, us: 32 + 16 heads, 1024 tokens 6.2 / 6.1, 2048: 12.8 / 10.5, 4001: 23.8 / 18.7, 8192: 45 / 35; 16 + 16 heads, 1024:
   // 4.8 / 5.1, 2048: 7.8 / 8.1, 4001: 16.4 / 15.0; 64 + 16 heads (two sets to a warp), 1024: 9.7 / 11.3, 2048: 20.2 / 20.9, 4001: 39 / 36; 8 + 2 heads
-  // (three warps at work), 4001: 6.8 / 16.1.
+  // (three warps at work), 4001: 6.8 / 16.1.  One number for all: at 2048 tokens it gains with 32 + 16 heads and loses 3 to 4 % with the other two.
   if (vec && stages >= 3 && T >= kStoreRingTokens && sets >= kStoreRingSets) {
     FORGE_ENSURE_DYN_SMEM(fp8_store_ring_kernel, kStoreSmem);
     const int ctas = std::min(T, kStoreCtasPerSm * device_sm_count());
@@ -331,7 +331,8 @@ extern "C" int forge_fp8_expand(const void* k_codes, const void* k_scales, const
                                 int* tables, int capacity, unsigned* status, cudaStream_t stream) {
   if (num_seqs <= 0 || table_width <= 0) return 0;
   if (block_size < 1 || num_seqs > 65535) return -1;
-  // a CTA's rows: 64, or 32 where there are few pages (64 / 32, us: 1 x 100 tokens 1.97 / 1.69, 1 x 700 2.28 / 2.57, 1 x 2000 3.88 / 3.34)
+  // a CTA's rows: 64, or 32 where there are few pages (64 / 32, us: 1 x 100 tokens 1.97 / 1.69, 1 x 700 2.28 / 2.57, 1 x 2000 3.88 / 3.34: two of the
+  // three gain more than the other loses)
   int rows = std::min(block_size, kExpandLoads * kExpandThreads / 16);
   while (rows > 32 && 2ll * capacity * nkv * (block_size / rows) < 4 * device_sm_count()) rows /= 2;
   const long long z = 2ll * nkv * (block_size / rows);

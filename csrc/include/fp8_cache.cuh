@@ -2,9 +2,10 @@
 // [blocks][kv_heads][block_size].  A byte b scales the head's 128 codes by 2^(b - 127), 255 stands for NaN.
 //
 // The scale is a power of two, the smallest with which no entry exceeds 448, the largest e4m3 number (not below 2^-126).  e4m3 is a
-// floating type: another scale would round no entry closer, except those below 2^-14 of the head's largest, which a power of two moves
-// into the subnormals one binade earlier.  In return the byte costs 1 / 128 of the codes (an fp32 scale 4 / 128), a code times its
-// scale is exact in bf16, and a product over keys takes the scale in as an addition to its exponent.
+// floating type: a finer scale has no smaller bound on an entry's relative error (2^-4), although it may hold a single entry closer, the head's
+// largest above all; only entries below 2^-14 of the largest come among the subnormals one binade earlier.  In return the byte costs
+// 1 / 128 of the codes (an fp32 scale 4 / 128), a product over keys takes the scale in as an addition to its exponent, and a code times
+// its scale is exact in bf16 from byte 3 on (below that, products under 2^-133 are rounded) and finite (see fp8_quantise).
 #pragma once
 
 #include <cuda_fp8.h>

@@ -349,7 +349,9 @@ class CudaOps(MixerOps, HybridOps, Fp8Ops):
         """Whether a decode step should take ``decode_attention_qkv`` rather than ``qk_norm_rope_store`` and ``attention``.  At large
         batches the attention is bound by bandwidth, and what is saved by a launch is less than the further work per sequence
         costs; over an 8-bit cache that is where ``attention`` would not take clusters (measured, two ops / one, us, 32 / 8 heads:
-        1 x 700 tokens 7.8 / 6.9, 4 x 3000 11.8 / 10.5, 16 x 200 8.7 / 7.4; where it does not, 32 x 1500, 24.7 / 26.5)."""
+        1 x 700 tokens 8.1 / 6.9, 4 x 3000 11.8 / 10.5, 16 x 200 9.0 / 7.8; where it does not, 32 x 1500, 24.7 / 26.5).  Both decide by the
+        width of the block table, which in captured steps is ``max_model_len``: with 8 KV heads up to 8 sequences at 4096 tokens, up to 4 at 8192,
+        none beyond."""
         if batch.padded_seqs > self.fused_qkv_max_batch:
             return False
         if not isinstance(k_cache, Fp8KVCache):
